@@ -115,6 +115,16 @@ SIGNATURES = {
     "ember_attn_decode_workspace_bytes": (sz, [i64, i64, i64, i64, i64, i64]),
     "ember_attn_decode": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64,
                                 f32, vp, sz, vp]),
+    "ember_kv4_write": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, vp]),
+    "ember_kv4_read_expanded": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp]),
+    "ember_attn_kv4_workspace_bytes": (sz, [i64, i64, i64, i64, i64, i64]),
+    "ember_attn_kv4": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, f32,
+                             vp, sz, vp]),
+    "ember_q8_code_bytes": (sz, [i64, i64]),
+    "ember_q8_param_bytes": (sz, [i64, i64]),
+    "ember_q8_quantize": (i32, [vp, vp, vp, i64, i64, vp]),
+    "ember_q8_dequantize": (i32, [vp, vp, vp, i64, i64, vp]),
+    "ember_q8_dequantize_rmsnorm": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, f32, vp]),
     "ember_argmax_rows": (i32, [vp, i64, i64, vp, vp]),
     "ember_argmax_rows_workspace_bytes": (sz, [i64, i64]),
     "ember_argmax_rows_ws": (i32, [vp, i64, i64, vp, vp, sz, vp]),

@@ -216,6 +216,29 @@ int ember_qknorm_rope_bwd(const float* dy, const float* x, const float* w, const
                           int64_t D, float eps, int64_t pos0, const float* freqs_host,
                           void* workspace, size_t workspace_bytes, ember_stream_t s);
 
+/* ------------------------------------------------- checkpoints in 8 bits
+ * Added in this build (the reference keeps the fp32 input of every
+ * checkpointed block, src/core/autograd.cu:327-363).  Rows [rows, H] in groups
+ * of 128 values (the last of a row may be shorter), each held as {lo, step}
+ * and one byte per value by the rule of ember_kv4_write with 255 steps.
+ * codes: rows of round_up(H, 16) bytes, the padding 0; params
+ * [rows][ceil(H/128)][2]; their sizes are ember_q8_code_bytes and
+ * ember_q8_param_bytes.  Any H; codes 16-byte and params 8-byte aligned
+ * (EMBER_EALIGN); fp32 rows that are not 16-byte aligned are accessed by
+ * single values.
+ * ember_q8_dequantize restores the rows; ember_q8_dequantize_rmsnorm also
+ * gives y = x * rstd * w, the restored rows' RMSNorm (rstd[rows] may be NULL),
+ * what a decoder block's re-run starts with. */
+size_t ember_q8_code_bytes(int64_t rows, int64_t H);
+size_t ember_q8_param_bytes(int64_t rows, int64_t H);
+int ember_q8_quantize(const float* x, void* codes, float* params, int64_t rows, int64_t H,
+                      ember_stream_t s);
+int ember_q8_dequantize(const void* codes, const float* params, float* x, int64_t rows, int64_t H,
+                        ember_stream_t s);
+int ember_q8_dequantize_rmsnorm(const void* codes, const float* params, const float* w, float* x,
+                                float* y, float* rstd, int64_t rows, int64_t H, float eps,
+                                ember_stream_t s);
+
 /* --------------------------------------------------------- elementwise
  * Replace src/ops/elementwise.cu:15-69, repeat_kv.cu:45-51 and
  * autograd.cu:88-93 (addinto). */
@@ -353,6 +376,44 @@ int ember_attn_decode(const float* q, const float* k, const float* v, float* o, 
                       int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t L, int64_t pos,
                       int64_t kv_sb, int64_t kv_sh, int64_t kv_st, float scale, void* workspace,
                       size_t workspace_bytes, ember_stream_t s);
+
+/* ---------------------------------------------------- KV cache in 4 bits
+ * Added in this build (the reference's cache is fp32).  A cache tensor is two
+ * buffers: codes [B, Hk, S, D/8], words of eight 4-bit codes with the first of
+ * them in the lowest bits, and params [B, Hk, S, 2] = {lo, step}, one pair per
+ * head row of D values.  A row is held as lo = its smallest value, step =
+ * (largest - smallest) / 15 rounded to fp32, and per value the code nearest
+ * (x - lo) / step; it reads back as fma(code, step, lo): at most step / 2 off,
+ * and exactly where all its values are equal.  A row with an infinity or a NaN
+ * reads back as NaN throughout.  Magnitudes below 2^127.
+ *
+ * ember_kv4_write quantises k and v [B,T,Hk,D] into rows [pos, pos+T) of their
+ * caches; EMBER_EINVAL unless 0 <= pos and pos + T <= S.
+ * ember_kv4_read_expanded: out [B, Hk*group, L, D] = what rows [0, L) of one
+ * cache tensor hold, KV head h/group for head h.
+ * D a multiple of 8 up to 256; codes and the fp32 tensors 16-byte aligned,
+ * params 8-byte aligned (EMBER_EALIGN). */
+int ember_kv4_write(const float* k, const float* v, uint32_t* k_codes, float* k_params,
+                    uint32_t* v_codes, float* v_params, int64_t B, int64_t T, int64_t Hk,
+                    int64_t D, int64_t S, int64_t pos, ember_stream_t s);
+int ember_kv4_read_expanded(const uint32_t* codes, const float* params, float* out, int64_t B,
+                            int64_t Hk, int64_t group, int64_t L, int64_t D, int64_t S,
+                            ember_stream_t s);
+/* ember_attn_decode over rows [0, L) of such a cache: q and o [B,T,H,D], query
+ * t sees rows j <= pos + t (and j < L), head h reads KV head h / (H/Hk), any T
+ * from one token to a chunk of a prompt.  The codes enter the products as they
+ * are held; sums and softmax statistics are fp32.  Rows past a query's last
+ * visible one do not reach its output, whatever they hold.  D in {64, 128};
+ * 1 <= L <= S < 2^31; alignment as above.  `workspace` >=
+ * ember_attn_kv4_workspace_bytes (0: none needed; EMBER_EWORKSPACE when
+ * smaller) holds the partial results of key splits, merged in a fixed order:
+ * deterministic. */
+size_t ember_attn_kv4_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
+                                      int64_t L);
+int ember_attn_kv4(const float* q, const uint32_t* k_codes, const float* k_params,
+                   const uint32_t* v_codes, const float* v_params, float* o, int64_t B, int64_t T,
+                   int64_t H, int64_t Hk, int64_t D, int64_t L, int64_t pos, int64_t S,
+                   float scale, void* workspace, size_t workspace_bytes, ember_stream_t s);
 
 /* ------------------------------------------------------ fused decode step
  * Kernels for calls of at most 8 token rows (decode), each streaming its
