@@ -199,31 +199,6 @@ __device__ __forceinline__ void wait_all_mem() {
   __builtin_amdgcn_s_waitcnt((7 << 4) | (0 << 8));
 }
 
-// Max and sum over lanes i, i + 16, i + 32, i + 48 of a wave, the four
-// 16-lane rows' values exchanged in registers: v_permlane16_swap trades rows
-// 1 and 3 of its first operand for rows 0 and 2 of its second, so with x in
-// both each lane holds x of rows {0, 1} or {2, 3}; v_permlane32_swap trades
-// the upper 32 lanes of the first for the lower 32 of the second.  max and +
-// of two operands are commutative, so every lane gets the same bits.
-__device__ __forceinline__ float pair_rows16(float x, bool sum) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
-  return sum ? a + b : fmaxf(a, b);
-}
-__device__ __forceinline__ float pair_rows32(float x, bool sum) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
-  return sum ? a + b : fmaxf(a, b);
-}
-__device__ __forceinline__ float max_over_rows(float x) {
-  return pair_rows32(pair_rows16(x, false), false);
-}
-__device__ __forceinline__ float sum_over_rows(float x) {
-  return pair_rows32(pair_rows16(x, true), true);
-}
-
 // ------------------------------------------------------------------ forward
 // Forward.  A wave owns 16 queries and a workgroup of eight waves 128 (of
 // four 64, see below), so every K/V tile in LDS serves them all, and at 100 registers per lane

@@ -102,11 +102,43 @@ __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
 }
 
 // ---------------------------------------------------------------- attention
-// Query rows of a KV head: r -> (t = r / G, h = hk*G + r % G), G = H / Hk.
-constexpr int kRowTile = 4;
-constexpr int kMinKeysPerSplit = 32;
-constexpr int kTargetBlocks = 512;
-constexpr int kMaxSplits = 1024;
+// Query rows of a KV head: r -> (t = r / G, h = hk*G + r % G), G = H / Hk.  A
+// group's rows share every code they unpack.
+//
+// Both products run on v_mfma_f32_16x16x32_f16 and lose nothing of the codes:
+// c - 8 is exact in f16, and the fp32 operand x beside it (a query, or a weight
+// times a step) is two f16 pieces, hi = f16(x) and lo = f16(x - hi), 22 bits of
+// it, so a product is two MFMAs into one fp32 accumulator.  Three bf16 pieces would
+// hold all 24 bits for half as many MFMAs again; the sums of D or L fp32 terms
+// around them round by more than the two bits.  With lo' = lo + 8 step,
+//   score_j = qmul (q' . (c_j - 8)) step_j + qsum lo'_j          (log2 units)
+// where q' = q 2^(15 - ex) is a query scaled by a power of two so that its
+// largest element lies in [2^14, 2^15): its low pieces then stay normal f16.
+// The softmax runs against a reference per query
+//   ref = max_j (score_j + e_j - 14),  2^e_j > step of value row j,
+// instead of max score_j, so that the weights p_j = 2^(score_j - ref) times
+// their steps stay below 2^14 and near it: the f16 range again, whatever the
+// rows' sizes.  e_j is at least -60, which bounds p_j by 2^74 where steps
+// vanish.  A query's bits depend on the rows it sees only.
+//
+// Fragments (lane = (g = lane / 16, i = lane % 16)):
+//   S^T = K Q^T: A holds key i, dims g D/4 + 8 s + {0,4,1,5,2,6,3,7} in step s (the
+//     order in which a word's codes unpack into f16 pairs), so a lane reads D/32
+//     consecutive words of one row; B holds query i's same dims; C holds keys
+//     4 g + e of query i.
+//   O^T += V^T P^T over 32 keys: B is P as it lies in the two C tiles, keys 16 kt
+//     + 4 g + e; A holds the same eight keys' codes at dim (D/16) i + t of tile t:
+//     the words of eight rows, paired by 16-bit halves, then unpacked as K's are;
+//     C holds dims (D/16)(4 g + e) + t of query i.
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlockKeys = 32;  // keys of one softmax step
+constexpr int kMaxSplits = 512;
+constexpr int64_t kMaxRows = 1 << 30;  // of a cache: row numbers are 32-bit in the kernels
 
 struct AttnArgs {
   const float* q;  // [B, T, H, D]
@@ -116,143 +148,623 @@ struct AttnArgs {
   const float* vp;
   float* o;        // [B, T, H, D]
   float* part_o;   // [B*T*H, nsplit, D]: each split's unnormalised sums
-  float* part_ml;  // [B*T*H, nsplit, 2]: its maximum (log2 units) and weight sum
-  int64_t T, H, Hk, L, pos, S;
-  int64_t kps;  // keys per split
+  float* part_ml;  // [B*T*H, nsplit, 2]: its reference (log2 units) and weight sum
+  int64_t T, H, Hk, pos, S;
+  int64_t heads;  // B * Hk
+  int L, kps;     // keys, and keys per split
   int nsplit, row_tiles;
   float qscale;  // scale * log2(e)
 };
 
-// A workgroup owns one (batch, KV head, row tile, key split); a key's words
-// lie over D/8 lanes, which form one group with an online softmax of its own.
-template <int D>
-__global__ __launch_bounds__(kThreads) void attn_kv4_kernel(AttnArgs a) {
-  constexpr int LPK = D / 8, KPW = kWave / LPK, NG = kWaves * KPW;
-  __shared__ float s_ml[NG][kRowTile][2];
-  __shared__ float s_o[NG][kRowTile][D];
-  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave;
-  const int w = lane % LPK, gid = wv * KPW + lane / LPK;
-  const int64_t G = a.H / a.Hk, R = G * a.T;
-  const int64_t split = blockIdx.x % a.nsplit, rest = blockIdx.x / a.nsplit;
-  const int64_t r0 = rest % a.row_tiles * kRowTile, bh = rest / a.row_tiles;
-  const int64_t hk = bh % a.Hk, b = bh / a.Hk;
-  const int64_t ks = split * a.kps, ke = ks + a.kps < a.L ? ks + a.kps : a.L;
-  const int nr = static_cast<int>(R - r0 < kRowTile ? R - r0 : kRowTile);
+__device__ __forceinline__ f32x4 mfma(half8_t a, half8_t b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 
-  float q[kRowTile][8], acc[kRowTile][8], m[kRowTile], l[kRowTile], qsum[kRowTile];
-  int64_t lim[kRowTile], jend = ks;
+// The eight codes of a word, less 8, in the order 0 4 1 5 2 6 3 7: bits of f16
+// 1024 + c and 1024 + 16 c, then exact arithmetic.
+__device__ __forceinline__ half8_t unpack8(uint32_t w) {
+  const half2_t k8 = {(_Float16)1032.f, (_Float16)1032.f};
+  const half2_t k72 = {(_Float16)72.f, (_Float16)72.f};
+  const half2_t k16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const uint32_t v = w >> 8;
+  const half2_t a = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) - k8;
+  const half2_t b = __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u) * k16 - k72;
+  const half2_t c = __builtin_bit_cast(half2_t, (v & 0x000f000fu) | 0x64006400u) - k8;
+  const half2_t d = __builtin_bit_cast(half2_t, (v & 0x00f000f0u) | 0x64006400u) * k16 - k72;
+  return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Low and high 16-bit halves of two words, a's below b's.
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// x as two f16 pieces.
+__device__ __forceinline__ void split_f16(const float (&x)[8], half8_t& hi, half8_t& lo) {
 #pragma unroll
-  for (int r = 0; r < kRowTile; ++r) {
-    m[r] = -INFINITY;
-    l[r] = qsum[r] = 0.f;
-    lim[r] = ks;
+  for (int e = 0; e < 8; ++e) {
+    hi[e] = static_cast<_Float16>(x[e]);
+    lo[e] = static_cast<_Float16>(x[e] - static_cast<float>(hi[e]));
+  }
+}
+
+// A query row's B fragments; rows that do not exist are zero.
+template <int D>
+struct QRow {
+  half8_t hi[D / 32], lo[D / 32];
+  float mul, sum;
+
+  __device__ __forceinline__ void load(const float* __restrict__ row, bool live, int g,
+                                       float qscale) {
+    float x[D / 4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[r][e] = acc[r][e] = 0.f;
-    if (r < nr) {
-      const int64_t t = (r0 + r) / G, h = hk * G + (r0 + r) % G;
-      const float* p = a.q + ((b * a.T + t) * a.H + h) * D + 8 * w;
+    for (int c = 0; c < D / 16; ++c) {
+      const f32x4 v = live ? reinterpret_cast<const f32x4*>(row + g * (D / 4))[c]
+                           : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        q[r][e] = p[e] * a.qscale;
-        qsum[r] += q[r][e];
-      }
-      const int64_t c = a.pos + t + 1;
-      lim[r] = c < ke ? c : ke;
-      jend = lim[r] > jend ? lim[r] : jend;
+      for (int e = 0; e < 4; ++e) x[4 * c + e] = v[e];
+    }
+    set(x, qscale);
+  }
+  // From the lane's D/4 values x of the row.
+  __device__ __forceinline__ void set(const float (&x)[D / 4], float qscale) {
+    float amax = 0.f, s = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 4; ++c) {
+      amax = fmaxf(amax, fabsf(x[c]));
+      s += x[c];
+    }
+    amax = max_over_rows(amax);
+    sum = sum_over_rows(s) * qscale;
+    const int ex = amax > 0.f && !not_finite(amax) ? __builtin_amdgcn_frexp_expf(amax) : 15;
+    mul = ldexpf(qscale, ex - 15);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[8 * k + (e >> 1) + 4 * (e & 1)], 15 - ex);
+      split_f16(y, hi[k], lo[k]);
     }
   }
-  for (int64_t j = ks + gid; j < jend; j += NG) {
-    const int64_t row = bh * a.S + j;
-    const uint32_t kw = a.kc[row * LPK + w], vw = a.vc[row * LPK + w];
-    const float2 kp = *reinterpret_cast<const float2*>(a.kp + 2 * row);
-    const float2 vp = *reinterpret_cast<const float2*>(a.vp + 2 * row);
-    float kx[8], vx[8];
+};
+
+// A query's running softmax; l and olo (sum p lo') are per lane until the end.
+struct Softmax {
+  float ref = -INFINITY, l = 0.f, olo = 0.f;
+};
+
+// The parameters of a block's keys in LDS, an array of KEYS floats each.
+enum { kKStep, kKLo, kVStep, kVLo, kVExp, kParams };
+
+// A key's or value's pair as those arrays hold it; absent rows get a step and
+// an offset of 0, and their scores are masked.
+template <int KEYS>
+__device__ __forceinline__ void stage_params(float* par, int key, bool value, float2 p, bool in) {
+  const float step = in ? p.y : 0.f;
+  const float lo8 = in ? fmaf(8.f, p.y, p.x) : 0.f;
+  par[(value ? kVStep : kKStep) * KEYS + key] = step;
+  par[(value ? kVLo : kKLo) * KEYS + key] = lo8;
+  if (value) {
+    const int ex = step > 0.f && !not_finite(step) ? __builtin_amdgcn_frexp_expf(step) : -60;
+    par[kVExp * KEYS + key] = static_cast<float>((ex > -60 ? ex : -60) - 14);
+  }
+}
+
+// One block of 32 keys for one query tile: the products s[kt] become weights,
+// in place; returns what the accumulators are to be multiplied by.  par: the
+// block's first key in the arrays of KEYS floats.  vis: how many keys from
+// this lane's first (4 g) on the query sees; MASK: some query does not see all.
+template <int KEYS, bool MASK>
+__device__ __forceinline__ float soften(f32x4 (&s)[2], const float* par, int g, int vis, float qmul,
+                                        float qsum, Softmax& st) {
+  float z = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) kx[e] = static_cast<float>((kw >> (4 * e)) & 15u);
-    held8(vw, vp, vx);
+  for (int kt = 0; kt < 2; ++kt) {
+    const float* p = par + 16 * kt + 4 * g;
+    const f32x4 step = *reinterpret_cast<const f32x4*>(p + kKStep * KEYS);
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p + kKLo * KEYS);
+    const f32x4 ex = *reinterpret_cast<const f32x4*>(p + kVExp * KEYS);
 #pragma unroll
-    for (int r = 0; r < kRowTile; ++r) {
-      float d = 0.f;
+    for (int e = 0; e < 4; ++e) {
+      s[kt][e] = fmaf(s[kt][e] * qmul, step[e], qsum * lo[e]);
+      if (MASK && 16 * kt + e >= vis) s[kt][e] = -INFINITY;
+      z = fmaxf(z, s[kt][e] + ex[e]);
+    }
+  }
+  const float ref = fmaxf(st.ref, max_over_rows(z));
+  // no key seen yet: any finite reference gives weights of 0
+  const float r = ref == -INFINITY ? 0.f : ref;
+  const float alpha = __builtin_amdgcn_exp2f(st.ref - r);
+  float l = 0.f, olo = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d = fmaf(q[r][e], kx[e], d);
-      float sc = fmaf(d, kp.y, qsum[r] * kp.x);
+  for (int kt = 0; kt < 2; ++kt) {
+    const float* p = par + 16 * kt + 4 * g;
+    const f32x4 step = *reinterpret_cast<const f32x4*>(p + kVStep * KEYS);
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p + kVLo * KEYS);
 #pragma unroll
-      for (int o = LPK / 2; o > 0; o >>= 1) sc += __shfl_xor(sc, o, kWave);
-      if (j < lim[r]) {
-        const float mx = fmaxf(m[r], sc);
-        const float c = exp2f(m[r] - mx), p = exp2f(sc - mx);
-        l[r] = l[r] * c + p;
+    for (int e = 0; e < 4; ++e) {
+      const bool hidden = MASK && 16 * kt + e >= vis;
+      const float w = __builtin_amdgcn_exp2f(s[kt][e] - r);
+      l += w;
+      // a row that the query does not see may hold NaN
+      olo = hidden ? olo : fmaf(w, lo[e], olo);
+      s[kt][e] = hidden ? 0.f : w * step[e];
+    }
+  }
+  st.l = st.l * alpha + l;
+  st.olo = st.olo * alpha + olo;
+  st.ref = ref;
+  return alpha;
+}
+
+__device__ __forceinline__ void weights(const f32x4 (&s)[2], half8_t& hi, half8_t& lo) {
+  const float x[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
+  split_f16(x, hi, lo);
+}
+
+// The weight of a partial result with reference m and weight sum l against M.
+// Rows whose scores are all NaN leave m = -inf and l = NaN.
+__device__ __forceinline__ float merge_weight(float m, float l, float M) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : l) : __builtin_amdgcn_exp2f(m - M);
+}
+
+// Block order: heads first, so that with 8 of them (or a multiple) a head's
+// blocks share one XCD's L2; then splits; row tiles last, the longest first.
+struct Item {
+  int64_t bh;
+  int split, tile;
+};
+__device__ __forceinline__ Item attn_item(const AttnArgs& a) {
+  const int64_t x = blockIdx.x;
+  const int64_t rest = x / a.heads;
+  return Item{x % a.heads, static_cast<int>(rest % a.nsplit),
+              a.row_tiles - 1 - static_cast<int>(rest / a.nsplit)};
+}
+
+// Few query rows: a workgroup owns up to 16 NT rows of one KV head and one key
+// split; its four waves take every fourth block of 32 keys, unpack their own
+// codes and are merged through LDS.  The next block's loads (five or so per
+// lane: K as fragments, V as 16-byte pieces that pass through LDS for their
+// transpose, one pair of parameters) are in flight during a block.
+template <int D, int NT>
+__global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
+  constexpr int W = D / 8, S = D / 32, ND = D / 16, ROWS = 16 * NT;
+  constexpr int VS = W + 4;                       // words per V row in LDS
+  constexpr int VP = kBlockKeys * W / 4 / kWave;  // 16-byte pieces of V per lane
+  constexpr int kStage = kBlockKeys * VS + kParams * kBlockKeys;  // per wave, words
+  constexpr int OS = D + 4;
+  constexpr int kMerge = kWaves * ROWS * (OS + 2);
+  constexpr int kLds = kWaves * kStage > kMerge ? kWaves * kStage : kMerge;
+  __shared__ __attribute__((aligned(16))) float lds[kLds];
+
+  const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const Item it = attn_item(a);
+  const int64_t hk = it.bh % a.Hk, b = it.bh / a.Hk;
+  const int G = static_cast<int>(a.H / a.Hk);
+  const int64_t R = G * a.T, r0 = static_cast<int64_t>(it.tile) * ROWS;
+  const int nr = static_cast<int>(R - r0 < ROWS ? R - r0 : ROWS);
+  const int ks = it.split * a.kps;
+  const int ke = a.L - ks < a.kps ? a.L : ks + a.kps;
+  // Keys [ks, jend) are seen by some row, [ks, jall) by every one.
+  const int64_t last = a.pos + (r0 + nr - 1) / G + 1, first = a.pos + r0 / G + 1;
+  const int jend = static_cast<int>(last < ke ? last : ke);
+  const int jall = static_cast<int>(first < ke ? first : ke);
+
+  uint32_t* vbuf = reinterpret_cast<uint32_t*>(lds) + w * kStage;
+  float* par = lds + w * kStage + kBlockKeys * VS;
+  const uint32_t* kc = a.kc + it.bh * a.S * W;
+  const uint32_t* vc = a.vc + it.bh * a.S * W;
+  const float2* pp = reinterpret_cast<const float2*>(lane < 32 ? a.kp : a.vp) + it.bh * a.S;
+
+  u32x4 kw[2], vw[VP];
+  float2 pw;
+  auto load = [&](int j0) {  // rows past the last key read that one again
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[r][e] = acc[r][e] * c + p * vx[e];
-        m[r] = mx;
+    for (int kt = 0; kt < 2; ++kt) {
+      const int64_t row = min(j0 + 16 * kt + i, a.L - 1);
+      const uint32_t* p = kc + row * W + g * S;
+      if constexpr (S == 4) {
+        kw[kt] = *reinterpret_cast<const u32x4*>(p);
+      } else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        kw[kt] = u32x4{x[0], x[1], 0u, 0u};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < VP; ++u) {
+      const int c = lane + kWave * u;
+      const int64_t row = min(j0 + c / (W / 4), a.L - 1);
+      vw[u] = *reinterpret_cast<const u32x4*>(vc + row * W + 4 * (c % (W / 4)));
+    }
+    pw = pp[min(j0 + (lane & 31), a.L - 1)];
+  };
+  const int j_first = ks + kBlockKeys * w;
+  if (j_first < jend) load(j_first);
+
+  QRow<D> q[NT];
+  int lim[NT];  // keys j < lim are seen; rows that do not exist see all
+  Softmax st[NT];
+  f32x4 acc[NT][ND];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = 16 * n + i;
+    const int64_t t = (r0 + r) / G, h = hk * G + (r0 + r) % G;
+    const bool live = r < nr;
+    q[n].load(a.q + (live ? ((b * a.T + t) * a.H + h) * D : 0), live, g, a.qscale);
+    const int64_t c = a.pos + t + 1;
+    lim[n] = live ? static_cast<int>(c < ke ? c : ke) : 0x7fffffff;
+#pragma unroll
+    for (int t2 = 0; t2 < ND; ++t2) acc[n][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int j0 = j_first; j0 < jend; j0 += kBlockKeys * kWaves) {
+    half8_t kf[2][S];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int k = 0; k < S; ++k) kf[kt][k] = unpack8(kw[kt][k]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = 0; u < VP; ++u) {
+      const int c = lane + kWave * u;
+      *reinterpret_cast<u32x4*>(vbuf + (c / (W / 4)) * VS + 4 * (c % (W / 4))) = vw[u];
+    }
+    stage_params<kBlockKeys>(par, lane & 31, lane >= 32, pw, j0 + (lane & 31) < jend);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (j0 + kBlockKeys * kWaves < jend) load(j0 + kBlockKeys * kWaves);
+
+    half8_t ph[NT], pl[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int k = 0; k < S; ++k)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          s[kt] = mfma(kf[kt][k], q[n].hi[k], s[kt]);
+          s[kt] = mfma(kf[kt][k], q[n].lo[k], s[kt]);
+        }
+      const int vis = lim[n] - j0 - 4 * g;
+      const float alpha =
+          j0 + kBlockKeys > jall
+              ? soften<kBlockKeys, true>(s, par, g, vis, q[n].mul, q[n].sum, st[n])
+              : soften<kBlockKeys, false>(s, par, g, vis, q[n].mul, q[n].sum, st[n]);
+      weights(s, ph[n], pl[n]);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int t = 0; t < ND; ++t) acc[n][t] *= alpha;
+      }
+    }
+    // V words of this lane's eight keys, then a half (D = 128: both) of each.
+    uint32_t vx[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      vx[e] = vbuf[(16 * (e >> 2) + 4 * g + (e & 3)) * VS + (D == 128 ? i : i >> 1)];
+#pragma unroll
+    for (int half = 0; half < ND / 4; ++half) {
+      half8_t u[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t x = vx[2 * p], y = vx[2 * p + 1];
+        const bool high = D == 128 ? half == 1 : (i & 1) == 1;
+        u[p] = unpack8(high ? high_halves(x, y) : low_halves(x, y));
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        half8_t vf;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          vf[2 * p] = u[p][2 * t];
+          vf[2 * p + 1] = u[p][2 * t + 1];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][4 * half + t] = mfma(vf, ph[n], acc[n][4 * half + t]);
+          acc[n][4 * half + t] = mfma(vf, pl[n], acc[n][4 * half + t]);
+        }
       }
     }
   }
+
+  __syncthreads();  // the stages are read no more
+  float* so = lds;                        // [wave][row][OS]
+  float* sm = lds + kWaves * ROWS * OS;   // [wave][row][2]
 #pragma unroll
-  for (int r = 0; r < kRowTile; ++r) {
+  for (int n = 0; n < NT; ++n) {
+    const float l = sum_over_rows(st[n].l), olo = sum_over_rows(st[n].olo);
+    const int row = w * ROWS + 16 * n + i;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s_o[gid][r][8 * w + e] = acc[r][e];
-    if (w == 0) {
-      s_ml[gid][r][0] = m[r];
-      s_ml[gid][r][1] = l[r];
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t4 = 0; t4 < ND / 4; ++t4) {
+        const f32x4 v = {acc[n][4 * t4][e], acc[n][4 * t4 + 1][e], acc[n][4 * t4 + 2][e],
+                         acc[n][4 * t4 + 3][e]};
+        *reinterpret_cast<f32x4*>(so + row * OS + ND * (4 * g + e) + 4 * t4) = v + olo;
+      }
+    if (g == 0) {
+      sm[2 * row] = st[n].ref;
+      sm[2 * row + 1] = l;
     }
   }
   __syncthreads();
-  for (int it = threadIdx.x; it < nr * D; it += kThreads) {
-    const int r = it / D, d = it % D;
+  for (int x = threadIdx.x; x < nr * (D / 4); x += kThreads) {
+    const int row = x / (D / 4), c4 = x % (D / 4);
     float M = -INFINITY;
-    for (int g = 0; g < NG; ++g) M = fmaxf(M, s_ml[g][r][0]);
-    float ls = 0.f, os = 0.f;
-    for (int g = 0; g < NG; ++g) {
-      const float e = s_ml[g][r][0] == -INFINITY ? 0.f : exp2f(s_ml[g][r][0] - M);
-      ls += s_ml[g][r][1] * e;
-      os += s_o[g][r][d] * e;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) M = fmaxf(M, sm[2 * (v * ROWS + row)]);
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const int at = v * ROWS + row;
+      const float e = merge_weight(sm[2 * at], sm[2 * at + 1], M);
+      l += sm[2 * at + 1] * e;
+      o += *reinterpret_cast<const f32x4*>(so + at * OS + 4 * c4) * e;
     }
-    const int64_t t = (r0 + r) / G, h = hk * G + (r0 + r) % G;
+    const int64_t t = (r0 + row) / G, h = hk * G + (r0 + row) % G;
     const int64_t orow = (b * a.T + t) * a.H + h;
     if (a.nsplit == 1) {
-      a.o[orow * D + d] = os / ls;
+      *reinterpret_cast<f32x4*>(a.o + orow * D + 4 * c4) = o * (1.f / l);
     } else {
-      a.part_o[(orow * a.nsplit + split) * D + d] = os;
-      if (d == 0) {
-        a.part_ml[(orow * a.nsplit + split) * 2] = M;
-        a.part_ml[(orow * a.nsplit + split) * 2 + 1] = ls;
+      *reinterpret_cast<f32x4*>(a.part_o + (orow * a.nsplit + it.split) * D + 4 * c4) = o;
+      if (c4 == 0) {
+        a.part_ml[(orow * a.nsplit + it.split) * 2] = M;
+        a.part_ml[(orow * a.nsplit + it.split) * 2 + 1] = l;
       }
     }
   }
 }
 
-// Merges a row's splits in split order: a block per row, D threads.
-__global__ void attn_kv4_combine(const float* __restrict__ part_o,
-                                 const float* __restrict__ part_ml, float* __restrict__ o,
-                                 int nsplit, int D) {
-  const int64_t row = blockIdx.x;
-  const float* ml = part_ml + row * nsplit * 2;
-  float M = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) M = fmaxf(M, ml[2 * s]);
-  float ls = 0.f, os = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float e = ml[2 * s] == -INFINITY ? 0.f : exp2f(ml[2 * s] - M);
-    ls += ml[2 * s + 1] * e;
-    os += part_o[(row * nsplit + s) * D + threadIdx.x] * e;
+// Many query rows: a workgroup owns 128 rows, 32 to a wave, and one key split.
+// Tiles of 64 keys are unpacked once, each wave a quarter, into two LDS
+// buffers that hold them as fragments, 16 bytes per lane one after another, so
+// that every wave's reads are free of bank conflicts; the next tile's codes are
+// loaded during a tile and unpacked after it.
+constexpr int kWideRows = 128;
+constexpr int kTileKeys = 64;
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
+  constexpr int W = D / 8, S = D / 32, ND = D / 16, NT = 2;
+  __shared__ half8_t kfrag[2][kTileKeys / 16][S][kWave];
+  __shared__ half8_t vfrag[2][kTileKeys / 32][ND][kWave];
+  __shared__ __attribute__((aligned(16))) float par[2][kParams * kTileKeys];
+
+  const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const Item it = attn_item(a);
+  const int64_t hk = it.bh % a.Hk, b = it.bh / a.Hk;
+  const int G = static_cast<int>(a.H / a.Hk);
+  const int64_t R = G * a.T, r0 = static_cast<int64_t>(it.tile) * kWideRows;
+  const int64_t rend = R - r0 < kWideRows ? R : r0 + kWideRows;
+  const int ks = it.split * a.kps;
+  const int ke = a.L - ks < a.kps ? a.L : ks + a.kps;
+  auto clip = [&](int64_t c) { return static_cast<int>(c < ke ? c : ke); };
+  const int jend = clip(a.pos + (rend - 1) / G + 1);
+  // This wave's rows, and the keys that some and all of them see.
+  const int64_t wr0 = r0 + 32 * w, wrend = rend - wr0 < 32 ? rend : wr0 + 32;
+  const int wend = wr0 < rend ? clip(a.pos + (wrend - 1) / G + 1) : ks;
+  const int wall = wr0 < rend ? clip(a.pos + wr0 / G + 1) : ks;
+
+  const uint32_t* kc = a.kc + it.bh * a.S * W;
+  const uint32_t* vc = a.vc + it.bh * a.S * W;
+  const float2* pp = reinterpret_cast<const float2*>(w == 0 ? a.kp : a.vp) + it.bh * a.S;
+
+  u32x4 kw;
+  uint32_t vw[4];
+  float2 pw = {0.f, 0.f};
+  auto load = [&](int j0) {  // rows past the last key read that one again
+    const int64_t row = min(j0 + 16 * w + i, a.L - 1);
+    const uint32_t* p = kc + row * W + g * S;
+    if constexpr (S == 4) {
+      kw = *reinterpret_cast<const u32x4*>(p);
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      kw = u32x4{x[0], x[1], 0u, 0u};
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t vrow = min(j0 + 16 * w + 4 * g + e, a.L - 1);
+      vw[e] = vc[vrow * W + (D == 128 ? i : i >> 1)];
+    }
+    if (w < 2) pw = pp[min(j0 + lane, a.L - 1)];
+  };
+  auto stage = [&](int buf, int j0) {
+#pragma unroll
+    for (int k = 0; k < S; ++k) kfrag[buf][w][k][lane] = unpack8(kw[k]);
+#pragma unroll
+    for (int half = 0; half < ND / 4; ++half) {
+      const bool high = D == 128 ? half == 1 : (i & 1) == 1;
+      const half8_t x = unpack8(high ? high_halves(vw[0], vw[1]) : low_halves(vw[0], vw[1]));
+      const half8_t y = unpack8(high ? high_halves(vw[2], vw[3]) : low_halves(vw[2], vw[3]));
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        reinterpret_cast<half4_t*>(&vfrag[buf][w >> 1][4 * half + t][lane])[w & 1] =
+            half4_t{x[2 * t], x[2 * t + 1], y[2 * t], y[2 * t + 1]};
+    }
+    if (w < 2) stage_params<kTileKeys>(par[buf], lane, w == 1, pw, j0 + lane < jend);
+  };
+
+  if (ks < jend) load(ks);
+  QRow<D> q[NT];
+  int lim[NT];
+  Softmax st[NT];
+  f32x4 acc[NT][ND];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t r = wr0 + 16 * n + i;
+    const int64_t t = r / G, h = hk * G + r % G;
+    const bool live = r < rend;
+    q[n].load(a.q + (live ? ((b * a.T + t) * a.H + h) * D : 0), live, g, a.qscale);
+    lim[n] = live ? clip(a.pos + t + 1) : 0x7fffffff;
+#pragma unroll
+    for (int t2 = 0; t2 < ND; ++t2) acc[n][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  o[row * D + threadIdx.x] = os / ls;
+  if (ks < jend) stage(0, ks);
+  __syncthreads();
+
+  int buf = 0;
+  for (int j0 = ks; j0 < jend; j0 += kTileKeys, buf ^= 1) {
+    const bool more = j0 + kTileKeys < jend;
+    if (more) load(j0 + kTileKeys);
+#pragma unroll
+    for (int u = 0; u < kTileKeys / 32; ++u) {
+      const int jb = j0 + 32 * u;
+      if (jb >= wend) continue;
+      f32x4 s[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[n][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < S; ++k)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          const half8_t kf = kfrag[buf][2 * u + kt][k][lane];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            s[n][kt] = mfma(kf, q[n].hi[k], s[n][kt]);
+            s[n][kt] = mfma(kf, q[n].lo[k], s[n][kt]);
+          }
+        }
+      half8_t ph[NT], pl[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float* pb = par[buf] + 32 * u;
+        const int vis = lim[n] - jb - 4 * g;
+        const float alpha =
+            jb + 32 > wall
+                ? soften<kTileKeys, true>(s[n], pb, g, vis, q[n].mul, q[n].sum, st[n])
+                : soften<kTileKeys, false>(s[n], pb, g, vis, q[n].mul, q[n].sum, st[n]);
+        weights(s[n], ph[n], pl[n]);
+        if (__any(alpha != 1.f)) {
+#pragma unroll
+          for (int t = 0; t < ND; ++t) acc[n][t] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        const half8_t vf = vfrag[buf][u][t][lane];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][t] = mfma(vf, ph[n], acc[n][t]);
+          acc[n][t] = mfma(vf, pl[n], acc[n][t]);
+        }
+      }
+    }
+    if (more) stage(buf ^ 1, j0 + kTileKeys);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float l = sum_over_rows(st[n].l), olo = sum_over_rows(st[n].olo);
+    const int64_t r = wr0 + 16 * n + i;
+    if (r >= rend) continue;
+    const int64_t t = r / G, h = hk * G + r % G;
+    const int64_t orow = (b * a.T + t) * a.H + h;
+    const float mul = a.nsplit == 1 ? 1.f / l : 1.f;
+    float* out = a.nsplit == 1 ? a.o + orow * D
+                               : a.part_o + (orow * a.nsplit + it.split) * D;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t4 = 0; t4 < ND / 4; ++t4) {
+        const f32x4 v = {acc[n][4 * t4][e], acc[n][4 * t4 + 1][e], acc[n][4 * t4 + 2][e],
+                         acc[n][4 * t4 + 3][e]};
+        *reinterpret_cast<f32x4*>(out + ND * (4 * g + e) + 4 * t4) = (v + olo) * mul;
+      }
+    if (a.nsplit > 1 && g == 0) {
+      a.part_ml[(orow * a.nsplit + it.split) * 2] = st[n].ref;
+      a.part_ml[(orow * a.nsplit + it.split) * 2 + 1] = l;
+    }
+  }
 }
 
+// Merges a row's splits in split order: a wave per row.  The splits' weights
+// are formed a lane each and kept in LDS, so the loop over splits only streams
+// partial rows.
+template <int D>
+__global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __restrict__ part_o,
+                                                             const float* __restrict__ part_ml,
+                                                             float* __restrict__ o, int64_t rows,
+                                                             int nsplit) {
+  constexpr int PER = D / kWave;
+  __shared__ float s_e[kWaves][kMaxSplits];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + w;
+  if (row >= rows) return;  // whole waves leave; no block barrier follows
+  const float* ml = part_ml + row * nsplit * 2;
+  float M = -INFINITY;
+  for (int s = lane; s < nsplit; s += kWave) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
+  float l = 0.f;
+  for (int s = lane; s < nsplit; s += kWave) {
+    const float e = merge_weight(ml[2 * s], ml[2 * s + 1], M);
+    s_e[w][s] = e;
+    l += ml[2 * s + 1] * e;
+  }
+  l = wave_sum(l);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  float acc[PER] = {};
+  const float* po = part_o + row * nsplit * D + lane;
+  int s = 0;
+  for (; s + 8 <= nsplit; s += 8) {
+    float x[8][PER];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int p = 0; p < PER; ++p) x[u][p] = po[(s + u) * D + p * kWave];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int p = 0; p < PER; ++p) acc[p] += x[u][p] * s_e[w][s + u];
+  }
+  for (; s < nsplit; ++s)
+#pragma unroll
+    for (int p = 0; p < PER; ++p) acc[p] += po[s * D + p * kWave] * s_e[w][s];
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int p = 0; p < PER; ++p) o[row * D + p * kWave + lane] = acc[p] * inv;
+}
+
+// How a call is laid out.  Up to 16 rows a KV head (a decode step) one query
+// tile, up to kNarrowRows two, beyond that the shared tiles of 128 rows.  Keys
+// are split until there are kTargetBlocks workgroups, each with at least one
+// block of 32 keys per wave (narrow) or kWideKeys keys (wide).
+constexpr int64_t kNarrowRows = 64;
+constexpr int64_t kTargetBlocks = 512;
+constexpr int64_t kNarrowKeys = kBlockKeys * kWaves;
+constexpr int64_t kWideKeys = 512;
+
 struct Plan {
-  int nsplit, row_tiles;
-  int64_t kps;
+  int variant;  // 1, 2: narrow with that many query tiles; 0: wide
+  int nsplit;
+  int64_t row_tiles, kps;
 };
 
 Plan attn_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t L) {
-  const int64_t tiles = (H / Hk * T + kRowTile - 1) / kRowTile;
-  const int64_t heads = B * Hk * tiles;
-  int64_t want = (kTargetBlocks + heads - 1) / heads;
-  const int64_t most = (L + kMinKeysPerSplit - 1) / kMinKeysPerSplit;
-  if (want > most) want = most;
+  const int64_t R = H / Hk * T;
+  Plan p{};
+  p.variant = R <= 16 ? 1 : R <= kNarrowRows ? 2 : 0;
+  const int64_t rows = p.variant ? 16 * p.variant : kWideRows;
+  const int64_t unit = p.variant ? kNarrowKeys : kWideKeys;
+  p.row_tiles = (R + rows - 1) / rows;
+  const int64_t items = B * Hk * p.row_tiles;
+  int64_t want = (kTargetBlocks + items - 1) / items;
+  const int64_t units = (L + unit - 1) / unit;
+  if (want > units) want = units;
   if (want > kMaxSplits) want = kMaxSplits;
-  const int64_t kps = (L + want - 1) / want;
-  return Plan{static_cast<int>((L + kps - 1) / kps), static_cast<int>(tiles), kps};
+  p.kps = (units + want - 1) / want * unit;
+  p.nsplit = static_cast<int>((L + p.kps - 1) / p.kps);
+  return p;
 }
 
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
@@ -315,18 +827,18 @@ extern "C" int ember_attn_kv4(const float* q, const uint32_t* k_codes, const flo
   if (B < 0 || T < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || pos < 0) return EMBER_EINVAL;
   if (D != 64 && D != 128) return EMBER_EINVAL;
   if (B == 0 || T == 0) return EMBER_OK;
-  if (L < 1 || L > S || S > 0x7fffffff) return EMBER_EINVAL;
+  if (L < 1 || L > S || S > kMaxRows || pos > kMaxRows) return EMBER_EINVAL;
   if (!q || !k_codes || !k_params || !v_codes || !v_params || !o) return EMBER_EINVAL;
   if (!aligned16(q) || !aligned16(o) || !aligned16(k_codes) || !aligned16(v_codes) ||
       !aligned8(k_params) || !aligned8(v_params))
     return EMBER_EALIGN;
   const Plan p = attn_plan(B, T, H, Hk, L);
   const int64_t blocks = B * Hk * p.row_tiles * p.nsplit;
-  if (blocks > 0x7fffffff) return EMBER_EINVAL;
+  const int64_t rows = B * T * H;
+  if (blocks > 0x7fffffff || rows > 0x7fffffff || p.kps > 0x7fffffff) return EMBER_EINVAL;
   const size_t need = ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, L);
   if (need && (!workspace || workspace_bytes < need)) return EMBER_EWORKSPACE;
   if (need && !aligned16(workspace)) return EMBER_EALIGN;
-  const int64_t rows = B * T * H;
   AttnArgs a{};
   a.q = q;
   a.kc = k_codes;
@@ -339,22 +851,30 @@ extern "C" int ember_attn_kv4(const float* q, const uint32_t* k_codes, const flo
   a.T = T;
   a.H = H;
   a.Hk = Hk;
-  a.L = L;
   a.pos = pos;
   a.S = S;
-  a.kps = p.kps;
+  a.heads = B * Hk;
+  a.L = static_cast<int>(L);
+  a.kps = static_cast<int>(p.kps);
   a.nsplit = p.nsplit;
-  a.row_tiles = p.row_tiles;
+  a.row_tiles = static_cast<int>(p.row_tiles);
   a.qscale = scale * 1.4426950408889634f;
   hipStream_t st = as_stream(s);
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (D == 128)
-    attn_kv4_kernel<128><<<grid, kThreads, 0, st>>>(a);
-  else
-    attn_kv4_kernel<64><<<grid, kThreads, 0, st>>>(a);
-  const int rc = launch_status();
-  if (rc || p.nsplit == 1) return rc;
-  attn_kv4_combine<<<static_cast<unsigned>(rows), static_cast<unsigned>(D), 0, st>>>(
-      a.part_o, a.part_ml, o, p.nsplit, static_cast<int>(D));
-  return launch_status();
+  auto launch = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.variant == 1)
+      attn_kv4_narrow<DD, 1><<<grid, kThreads, 0, st>>>(a);
+    else if (p.variant == 2)
+      attn_kv4_narrow<DD, 2><<<grid, kThreads, 0, st>>>(a);
+    else
+      attn_kv4_wide<DD><<<grid, kThreads, 0, st>>>(a);
+    const int rc = launch_status();
+    if (rc || p.nsplit == 1) return rc;
+    attn_kv4_combine<DD><<<static_cast<unsigned>((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(
+        a.part_o, a.part_ml, o, rows, p.nsplit);
+    return launch_status();
+  };
+  return D == 128 ? launch(std::integral_constant<int, 128>{})
+                  : launch(std::integral_constant<int, 64>{});
 }

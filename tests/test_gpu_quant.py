@@ -102,11 +102,11 @@ def test_kv4_write_and_read(B, T, Hk, D, S, pos):
 
 
 # --------------------------------------------------------------------------- attention
-def held_cache(r, B, Hk, S, D, spread=1.0):
+def held_cache(r, B, Hk, S, D):
     """A cache's buffers (numpy) and the values it holds, in 64 bits."""
     out = []
     for _ in range(2):
-        codes, params = OQ.quantise(spread * rows_like_keys(r, B, Hk, S, D), 15)
+        codes, params = OQ.quantise(rows_like_keys(r, B, Hk, S, D), 15)
         out.append((OQ.pack4(codes), params, OQ.values(codes, params)))
     return out
 
@@ -242,6 +242,18 @@ def test_attention_rows_that_are_not_finite_reach_only_who_sees_them(T):
     got = attend(q, cache, L, L - T, 0.125)
     bad[0, T - 1, 1] = True
     assert np.isnan(got[bad]).all() and same(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("T", [1, 20, 90])
+def test_attention_whole_blocks_of_not_finite_rows(T):
+    """A split, or a wave's share of one, in which no score is a number still reaches the result."""
+    r = rng(7)
+    H, Hk, D, L = 2, 2, 128, 1700
+    q = r.standard_normal((1, T, H, D)).astype(np.float32)
+    cache = held_cache(r, 1, Hk, L, D)
+    cache[0][1][0, 1, 600:1300] = np.nan
+    got = attend(q, cache, L, L - T, 0.1)
+    assert np.isnan(got[:, :, 1]).all() and np.isfinite(got[:, :, 0]).all()
 
 
 @pytest.mark.parametrize("T,L", [(1, 3000), (3, 700), (96, 1200)])

@@ -76,7 +76,8 @@ def attn(B=1, T=1, H=4, Hk=2, D=64, L=4, pos=3, S=8, q=P, kc=P, kp=P, vc=P, vp=P
 
 def test_attention_refusals():
     assert attn(D=96) == -1 and attn(H=3) == -1 and attn(Hk=0) == -1 and attn(pos=-1) == -1
-    assert attn(L=0) == -1 and attn(L=9) == -1 and attn(S=2 ** 31, L=4) == -1
+    assert attn(L=0) == -1 and attn(L=9) == -1 and attn(S=2 ** 30 + 1, L=4) == -1
+    assert attn(pos=2 ** 30 + 1) == -1 and attn(pos=2 ** 63 - 1) == -1
     assert attn(B=-1) == -1 and attn(T=-1) == -1
     for name in ("q", "kc", "kp", "vc", "vp", "o"):
         assert attn(**{name: None}) == -1, name
