@@ -4,7 +4,7 @@
   compiled with hipcc for gfx950 only.
 * ``emberlm_amd/lib/libctd.so``        -- the C++ Tensor/autograd/Module/optim layer
   (include/ctd/...), host-only C++ that calls nothing but the C ABI.
-* ``emberlm_amd/lib/ctd_tests``        -- the C++ test binary (tests/cpp/*.cpp).
+* ``emberlm_amd/lib/ctd_tests``, ``ctd_quant_tests`` -- the C++ test binaries (tests/cpp/).
 
 Usage: ``python -m emberlm_amd.build`` (or ``__graft_entry__.build()``).
 """
@@ -96,20 +96,27 @@ def build_host(verbose=False):
 
 
 def build_cpp_tests(verbose=False):
-    srcs = sorted(glob.glob(os.path.join(ROOT, "tests", "cpp", "*.cpp")))
-    if not srcs or not os.path.exists(os.path.join(LIB, "libctd.so")):
-        return None
+    """The test programs: tests/cpp/*.cpp into lib/ctd_tests, tests/cpp/quant/*.cpp into
+    lib/ctd_quant_tests."""
+    if not os.path.exists(os.path.join(LIB, "libctd.so")):
+        return []
     cxx = shutil.which("g++") or "g++"
-    out = os.path.join(LIB, "ctd_tests")
     oracle_inc = os.path.join(ROOT, "oracle")
     oracle_lib = os.path.join(ROOT, "oracle", "_build")
-    _run([cxx, *CXX_FLAGS, "-I" + oracle_inc, "-o", out + ".tmp", *srcs, "-L" + LIB, "-lctd",
-          "-lember_hip", "-L" + oracle_lib, "-lember_oracle",
-          "-Wl,-rpath,$ORIGIN", "-Wl,-rpath,$ORIGIN/../../oracle/_build", "-lm"])
-    os.replace(out + ".tmp", out)
-    if verbose:
-        print("built", out)
-    return out
+    outs = []
+    for folder, name in ((".", "ctd_tests"), ("quant", "ctd_quant_tests")):
+        srcs = sorted(glob.glob(os.path.join(ROOT, "tests", "cpp", folder, "*.cpp")))
+        if not srcs:
+            continue
+        out = os.path.join(LIB, name)
+        _run([cxx, *CXX_FLAGS, "-I" + oracle_inc, "-o", out + ".tmp", *srcs, "-L" + LIB, "-lctd",
+              "-lember_hip", "-L" + oracle_lib, "-lember_oracle",
+              "-Wl,-rpath,$ORIGIN", "-Wl,-rpath,$ORIGIN/../../oracle/_build", "-lm"])
+        os.replace(out + ".tmp", out)
+        outs.append(out)
+        if verbose:
+            print("built", out)
+    return outs
 
 
 def build_tools(verbose=False):

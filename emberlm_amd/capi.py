@@ -120,6 +120,8 @@ SIGNATURES = {
     "ember_attn_kv4_workspace_bytes": (sz, [i64, i64, i64, i64, i64, i64]),
     "ember_attn_kv4": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, f32,
                              vp, sz, vp]),
+    "ember_attn_kv4_qkv": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, f32,
+                                 C.POINTER(f32), i64, vp, vp, vp, vp, i64, f32, vp, vp, sz, vp]),
     "ember_q8_code_bytes": (sz, [i64, i64]),
     "ember_q8_param_bytes": (sz, [i64, i64]),
     "ember_q8_quantize": (i32, [vp, vp, vp, i64, i64, vp]),

@@ -28,10 +28,13 @@
 #include <atomic>
 #include <queue>
 #include <stdexcept>
+#include <tuple>
+#include <utility>
 #include <string>
 #include <unordered_map>
 
 #include "ctd/autograd.h"
+#include "ctd/ops/quant.h"
 #include "ctd/runtime.h"
 #include "ember_hip.h"
 
@@ -318,6 +321,22 @@ void accumulate_inplace(Tensor& dst, const Tensor& src) {
 // ------------------------------------------------------------ checkpoint
 namespace {
 
+// The gradient of block's result at the leaf, from the result's gradient.
+template <typename Block>
+Tensor replay_gradient(Tensor leaf, const Block& block, const Tensor& grad_out) {
+  leaf.requires_grad_(true);
+  Tensor replay;
+  {
+    const GradModeScope tape_on(true);  // the replay must record, whatever the caller's mode
+    replay = block(leaf);
+  }
+  // The replay's graph is built afresh on every call, so its own pass never
+  // needs to keep it; the outer pass's setting decides whether the saved
+  // input stays for another recompute.
+  replay.backward(grad_out, false);
+  return leaf.grad();
+}
+
 // Keeps the block's input and function; its backward replays the function on
 // a fresh leaf copy of the input with the tape on, back-propagates the
 // incoming gradient through the replay (parameters accumulate their
@@ -330,18 +349,7 @@ class RecomputeNode final : public Node {
 
   std::vector<Tensor> backward(const std::vector<Tensor>& grads_out) override {
     if (grads_out.empty() || !grads_out[0].defined()) return {Tensor{}};
-    Tensor leaf = input_.detach();
-    leaf.requires_grad_(true);
-    Tensor replay;
-    {
-      const GradModeScope tape_on(true);  // the replay must record, whatever the caller's mode
-      replay = block_(leaf);
-    }
-    // The replay's graph is built afresh on every call, so its own pass never
-    // needs to keep it; the outer pass's setting decides whether the saved
-    // input stays for another recompute.
-    replay.backward(grads_out[0], false);
-    Tensor g = leaf.grad();
+    Tensor g = replay_gradient(input_.detach(), block_, grads_out[0]);
     if (!graph_retained()) input_ = Tensor{};  // the saved activation is not needed again
     return {g};
   }
@@ -351,7 +359,74 @@ class RecomputeNode final : public Node {
   Tensor input_;
 };
 
+// RecomputeNode with the input in 8 bits, restored for the replay, together
+// with its norm's values where a norm is given.
+class RecomputeQ8Node final : public Node {
+ public:
+  using Fn = std::function<Tensor(const Tensor&, const ops::NormValues*)>;
+  RecomputeQ8Node(Fn block, ops::Q8Rows input, Tensor norm_weight, float norm_eps)
+      : block_(std::move(block)),
+        input_(std::move(input)),
+        norm_weight_(std::move(norm_weight)),
+        norm_eps_(norm_eps) {}
+  const char* name() const override { return "CheckpointQ8Node"; }
+
+  std::vector<Tensor> backward(const std::vector<Tensor>& grads_out) override {
+    if (grads_out.empty() || !grads_out[0].defined()) return {Tensor{}};
+    Tensor x;
+    ops::NormValues values;
+    if (norm_weight_.defined())
+      std::tie(x, values) = ops::dequantize_q8_rms_norm(input_, norm_weight_, norm_eps_);
+    else
+      x = ops::dequantize_q8(input_);
+    if (!graph_retained()) input_ = {};  // restored for the last time
+    auto block = [&](const Tensor& leaf) {
+      // The block takes the values over, so that they die with its own use.
+      const ops::NormValues normed = std::exchange(values, {});
+      return block_(leaf, norm_weight_.defined() ? &normed : nullptr);
+    };
+    return {replay_gradient(std::move(x), block, grads_out[0])};
+  }
+
+ private:
+  Fn block_;
+  ops::Q8Rows input_;
+  Tensor norm_weight_;
+  float norm_eps_;
+};
+
+Tensor checkpoint_q8_with(RecomputeQ8Node::Fn fn, const Tensor& input, const Tensor& norm_weight,
+                          float norm_eps) {
+  if (!t_grad_mode) return fn(input, nullptr);
+  Tensor out;
+  ops::Q8Rows held;
+  {
+    const GradModeScope tape_off(false);
+    held = ops::quantize_q8(input);
+    out = fn(input, nullptr);
+  }
+  auto node = std::make_shared<RecomputeQ8Node>(std::move(fn), std::move(held),
+                                                norm_weight.detach(), norm_eps);
+  node->next_edges = collect_next_edges({input});
+  set_history(out, std::move(node));
+  return out;
+}
+
 }  // namespace
+
+Tensor checkpoint_q8(std::function<Tensor(const Tensor&)> fn, const Tensor& input) {
+  return checkpoint_q8_with(
+      [fn = std::move(fn)](const Tensor& x, const ops::NormValues*) { return fn(x); }, input,
+      Tensor{}, 0.0f);
+}
+
+Tensor checkpoint_q8(std::function<Tensor(const Tensor&, const ops::NormValues*)> fn,
+                     const Tensor& input, const Tensor& norm_weight, float norm_eps) {
+  if (!norm_weight.defined() || norm_weight.dim() != 1 || input.dim() < 1 ||
+      norm_weight.shape()[0] != input.shape().back())
+    throw std::runtime_error("checkpoint_q8: norm weight does not belong to the input");
+  return checkpoint_q8_with(std::move(fn), input, norm_weight, norm_eps);
+}
 
 Tensor checkpoint(std::function<Tensor(const Tensor&)> fn, const Tensor& input) {
   if (!t_grad_mode) return fn(input);

@@ -83,6 +83,11 @@ Request parse_request(const std::string& text) {
     r.thinking_token_budget = static_cast<int>(integer(*v, "thinking_token_budget"));
   if (const JVal* v = req.find("think_open_ids")) r.think_open_ids = ids(*v, "think_open_ids");
   if (const JVal* v = req.find("think_close_ids")) r.think_close_ids = ids(*v, "think_close_ids");
+  if (const JVal* v = req.find("kv_bits")) {
+    r.kv_bits = static_cast<int>(integer(*v, "kv_bits"));
+    if (r.kv_bits != 32 && r.kv_bits != 4)
+      throw std::runtime_error("request: kv_bits must be 32 or 4");
+  }
   return r;
 }
 
@@ -158,7 +163,8 @@ LoopResult generate_loop(const nn::Model& model, const Request& req,
     throw std::runtime_error("generate: need 1 <= prompt length < max_seq_len");
   const std::unordered_set<int64_t> eos(req.eos_ids.begin(), req.eos_ids.end());
   nn::KVCache cache = nn::KVCache::allocate(cfg.num_hidden_layers, cfg.num_key_value_heads,
-                                            cfg.head_dim, /*batch=*/1, req.max_seq_len, kHIP0);
+                                            cfg.head_dim, /*batch=*/1, req.max_seq_len, kHIP0,
+                                            req.kv_bits);
   ThinkBudget think(req);
   LoopResult res;
   res.reason = "max_tokens";

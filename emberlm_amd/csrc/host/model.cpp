@@ -155,6 +155,8 @@ namespace {
 
 // embedding -> blocks (checkpointed when enabled) -> final RMSNorm: [B, T, H].
 Tensor train_hidden(const Model& m, const Tensor& input_ids) {
+  if (m.checkpoint_bits != 32 && m.checkpoint_bits != 8)
+    throw std::runtime_error("Model: checkpoint_bits must be 32 or 8");
   Tensor h = m.embed_tokens.forward(input_ids);
   for (size_t i = 0; i < m.layers.size(); ++i) {
     const TransformerBlock& layer = m.layers[i];
@@ -163,6 +165,16 @@ Tensor train_hidden(const Model& m, const Tensor& input_ids) {
       // enabled when the backward pass re-runs it; the re-run only
       // back-propagates through its result, so the block skips computing it.
       const int li = static_cast<int>(i);
+      if (m.checkpoint_bits == 8) {
+        h = autograd::checkpoint_q8(
+            [&m, &layer, li](const Tensor& x, const ops::NormValues* normed) {
+              if (!autograd::is_grad_enabled()) return layer.forward_train(x);
+              if (m.recompute_hook) m.recompute_hook(li);
+              return layer.forward_train_for_backward(x, normed);
+            },
+            h, layer.input_layernorm.weight, layer.input_layernorm.eps);
+        continue;
+      }
       h = autograd::checkpoint(
           [&m, &layer, li](const Tensor& x) {
             if (!autograd::is_grad_enabled()) return layer.forward_train(x);

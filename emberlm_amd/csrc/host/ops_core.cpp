@@ -322,13 +322,23 @@ Tensor rms_norm(const Tensor& x, const Tensor& weight, float eps) {
   if (!autograd::any_requires_grad({x, weight})) return rms_norm_impl(x, weight, eps);
   const int64_t H = x.shape().back();
   const int64_t rows = x.numel() / H;
-  Tensor y = empty_like(x);
-  Tensor rstd = Tensor::empty({rows}, DType::kFloat32, x.device());
-  CTD_CHECK(ember_rmsnorm_fwd(cfp(x), cfp(weight), fp(y), fp(rstd), rows, H, eps, S()));
+  NormValues v{empty_like(x), Tensor::empty({rows}, DType::kFloat32, x.device())};
+  CTD_CHECK(ember_rmsnorm_fwd(cfp(x), cfp(weight), fp(v.y), fp(v.rstd), rows, H, eps, S()));
+  return rms_norm_from(x, weight, eps, v);
+}
+
+Tensor rms_norm_from(const Tensor& x, const Tensor& weight, float eps, const NormValues& values) {
+  check_norm(x, weight);
+  check_f32(values.y, "rms_norm_from", "y");
+  check_f32(values.rstd, "rms_norm_from", "rstd");
+  require(values.y.shape() == x.shape() && values.rstd.numel() * x.shape().back() == x.numel(),
+          "rms_norm_from: values of another shape");
+  Tensor y = values.y.detach();
+  if (!autograd::any_requires_grad({x, weight})) return y;
   auto node = std::make_shared<RmsNormBackward>();
   node->x = x.detach();
   node->w = weight.detach();
-  node->rstd = rstd;
+  node->rstd = values.rstd;
   node->eps = eps;
   node->next_edges = autograd::collect_next_edges({x, weight});
   autograd::set_history(y, std::move(node));

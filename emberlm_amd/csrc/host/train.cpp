@@ -152,6 +152,9 @@ Config load_config(const fs::path& cfg_path) {
   }
   c.offload_optimizer = get_bool(j, "offload_optimizer", c.offload_optimizer);
   c.gradient_checkpointing = get_bool(j, "gradient_checkpointing", c.gradient_checkpointing);
+  c.checkpoint_bits = get_int(j, "checkpoint_bits", c.checkpoint_bits);
+  if (c.checkpoint_bits != 32 && (c.checkpoint_bits != 8 || !c.gradient_checkpointing))
+    throw std::runtime_error("config: checkpoint_bits must be 32, or 8 with gradient_checkpointing");
   if (const json::JVal* m = key(j, "model")) {
     c.model = model_config(*m);
     c.has_model = true;
@@ -356,6 +359,7 @@ int run(const Config& cfg) {
   nn::Model model = nn::build_model(weights, arch);
   weights.clear();
   model.gradient_checkpointing = cfg.gradient_checkpointing;
+  model.checkpoint_bits = cfg.checkpoint_bits;
   auto named = model.collect_parameters();
   std::cerr << "ctd_train: " << named.all.size() << " parameter tensors (" << named.decay.size()
             << " with weight decay)\n";

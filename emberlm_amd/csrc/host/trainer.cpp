@@ -278,6 +278,13 @@ int ctd_trainer_get_grad(ctd_trainer_t t, int64_t i, float* host, int64_t numel)
   }
 }
 
+int ctd_trainer_set_checkpoint_bits(ctd_trainer_t t, int32_t bits) {
+  return guarded([&] {
+    if (bits != 32 && bits != 8) throw std::runtime_error("checkpoint bits must be 32 or 8");
+    as_trainer(t)->model.checkpoint_bits = bits;
+  });
+}
+
 int ctd_trainer_set_checkpointing(ctd_trainer_t t, int32_t on) {
   return guarded([&] { as_trainer(t)->model.gradient_checkpointing = on != 0; });
 }
@@ -367,7 +374,15 @@ int ctd_trainer_block_step(ctd_trainer_t t, int64_t layer, const float* x, const
       return autograd::is_grad_enabled() ? blk.forward_train_for_backward(v)
                                          : blk.forward_train(v);
     };
-    Tensor y = checkpoint ? autograd::checkpoint(fn, xin) : blk.forward_train(xin);
+    auto fn8 = [&blk](const Tensor& v, const ops::NormValues* normed) {
+      return autograd::is_grad_enabled() ? blk.forward_train_for_backward(v, normed)
+                                         : blk.forward_train(v);
+    };
+    Tensor y = !checkpoint                      ? blk.forward_train(xin)
+               : tr->model.checkpoint_bits == 8 ? autograd::checkpoint_q8(
+                                                      fn8, xin, blk.input_layernorm.weight,
+                                                      blk.input_layernorm.eps)
+                                                : autograd::checkpoint(fn, xin);
     if (y_out) y.copy_to_host(y_out);
     Tensor g = Tensor::from_host(dy, {B, T, d}, DType::kFloat32, kHIP0);
     y.backward(g);
@@ -724,13 +739,18 @@ int ctd_train_event_json(int32_t step, float loss, float lr, float grad_norm,
 }
 
 int ctd_kvcache_create(ctd_trainer_t t, int64_t batch, int64_t max_seq, ctd_kvcache_t* out) {
+  return ctd_kvcache_create_bits(t, batch, max_seq, 32, out);
+}
+
+int ctd_kvcache_create_bits(ctd_trainer_t t, int64_t batch, int64_t max_seq, int32_t bits,
+                            ctd_kvcache_t* out) {
   return guarded([&] {
     Trainer* tr = as_trainer(t);
     if (!out) throw std::runtime_error("null output handle");
     if (batch < 1 || max_seq < 1) throw std::runtime_error("kv cache: batch, max_seq >= 1");
     const nn::LlamaConfig& c = tr->model.config;
     *out = new nn::KVCache(nn::KVCache::allocate(c.num_hidden_layers, c.num_key_value_heads,
-                                                 c.head_dim, batch, max_seq, kHIP0));
+                                                 c.head_dim, batch, max_seq, kHIP0, bits));
   });
 }
 
@@ -777,6 +797,14 @@ int ctd_trainer_generate(ctd_trainer_t t, const int64_t* prompt, int64_t P, int3
                          float temperature, int32_t top_k, float top_p, uint64_t seed,
                          int64_t max_seq, int64_t* tokens, double* prefill_ms,
                          double* decode_ms) {
+  return ctd_trainer_generate_bits(t, prompt, P, max_new, temperature, top_k, top_p, seed, max_seq,
+                                   32, tokens, prefill_ms, decode_ms);
+}
+
+int ctd_trainer_generate_bits(ctd_trainer_t t, const int64_t* prompt, int64_t P, int32_t max_new,
+                              float temperature, int32_t top_k, float top_p, uint64_t seed,
+                              int64_t max_seq, int32_t kv_bits, int64_t* tokens,
+                              double* prefill_ms, double* decode_ms) {
   return guarded([&] {
     Trainer* tr = as_trainer(t);
     if (P < 1 || max_new < 0 || P + max_new > max_seq)
@@ -787,6 +815,7 @@ int ctd_trainer_generate(ctd_trainer_t t, const int64_t* prompt, int64_t P, int3
     req.max_seq_len = static_cast<int>(max_seq);
     req.sampler = SamplerConfig{temperature, top_k, top_p};
     req.seed = seed;
+    req.kv_bits = kv_bits;
     runtime::synchronize();
     int n = 0;
     const generate::LoopResult r =

@@ -149,9 +149,10 @@ struct AttnArgs {
   float* o;        // [B, T, H, D]
   float* part_o;   // [B*T*H, nsplit, D]: each split's unnormalised sums
   float* part_ml;  // [B*T*H, nsplit, 2]: its reference (log2 units) and weight sum
-  int64_t T, H, Hk, pos, S;
-  int64_t heads;  // B * Hk
-  int L, kps;     // keys, and keys per split
+  int64_t S;
+  unsigned heads;  // B * Hk
+  unsigned T, H, Hk, G;
+  int L, pos;
   int nsplit, row_tiles;
   float qscale;  // scale * log2(e)
 };
@@ -161,16 +162,23 @@ __device__ __forceinline__ f32x4 mfma(half8_t a, half8_t b, f32x4 c) {
 }
 
 // The eight codes of a word, less 8, in the order 0 4 1 5 2 6 3 7: bits of f16
-// 1024 + c and 1024 + 16 c, then exact arithmetic.
-__device__ __forceinline__ half8_t unpack8(uint32_t w) {
+// 1024 + c and 1024 + 16 c, then exact arithmetic.  `one` is 0x64006400 (two
+// f16 1024) in a register of its own: a mask and an or of two literals would be
+// two instructions.
+__device__ __forceinline__ uint32_t two_1024() {
+  uint32_t one = 0x64006400u;
+  asm("" : "+v"(one));
+  return one;
+}
+__device__ __forceinline__ half8_t unpack8(uint32_t w, uint32_t one) {
   const half2_t k8 = {(_Float16)1032.f, (_Float16)1032.f};
   const half2_t k72 = {(_Float16)72.f, (_Float16)72.f};
   const half2_t k16 = {(_Float16)0.0625f, (_Float16)0.0625f};
   const uint32_t v = w >> 8;
-  const half2_t a = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) - k8;
-  const half2_t b = __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u) * k16 - k72;
-  const half2_t c = __builtin_bit_cast(half2_t, (v & 0x000f000fu) | 0x64006400u) - k8;
-  const half2_t d = __builtin_bit_cast(half2_t, (v & 0x00f000f0u) | 0x64006400u) * k16 - k72;
+  const half2_t a = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | one) - k8;
+  const half2_t b = __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | one) * k16 - k72;
+  const half2_t c = __builtin_bit_cast(half2_t, (v & 0x000f000fu) | one) - k8;
+  const half2_t d = __builtin_bit_cast(half2_t, (v & 0x00f000f0u) | one) * k16 - k72;
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -182,12 +190,20 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// x as two f16 pieces.
+// x as two f16 pieces (pairs convert in one instruction).
+typedef float float2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split_f16(const float (&x)[8], half8_t& hi, half8_t& lo) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    hi[e] = static_cast<_Float16>(x[e]);
-    lo[e] = static_cast<_Float16>(x[e] - static_cast<float>(hi[e]));
+  for (int e = 0; e < 8; e += 2) {
+    const half2_t h = __builtin_convertvector((float2_t{x[e], x[e + 1]}), half2_t);
+    const half2_t l = __builtin_convertvector(
+        (float2_t{fmaf(static_cast<float>(h[0]), -1.f, x[e]),
+                  fmaf(static_cast<float>(h[1]), -1.f, x[e + 1])}),
+        half2_t);
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    lo[e] = l[0];
+    lo[e + 1] = l[1];
   }
 }
 
@@ -197,9 +213,9 @@ struct QRow {
   half8_t hi[D / 32], lo[D / 32];
   float mul, sum;
 
-  __device__ __forceinline__ void load(const float* __restrict__ row, bool live, int g,
-                                       float qscale) {
-    float x[D / 4];
+  // The lane's D/4 values of a row.
+  static __device__ __forceinline__ void load(const float* __restrict__ row, bool live, int g,
+                                              float (&x)[D / 4]) {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       const f32x4 v = live ? reinterpret_cast<const f32x4*>(row + g * (D / 4))[c]
@@ -207,9 +223,7 @@ struct QRow {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * c + e] = v[e];
     }
-    set(x, qscale);
   }
-  // From the lane's D/4 values x of the row.
   __device__ __forceinline__ void set(const float (&x)[D / 4], float qscale) {
     float amax = 0.f, s = 0.f;
 #pragma unroll
@@ -314,24 +328,147 @@ __device__ __forceinline__ float merge_weight(float m, float l, float M) {
 // Block order: heads first, so that with 8 of them (or a multiple) a head's
 // blocks share one XCD's L2; then splits; row tiles last, the longest first.
 struct Item {
-  int64_t bh;
-  int split, tile;
+  int bh, split, tile;
 };
 __device__ __forceinline__ Item attn_item(const AttnArgs& a) {
-  const int64_t x = blockIdx.x;
-  const int64_t rest = x / a.heads;
-  return Item{x % a.heads, static_cast<int>(rest % a.nsplit),
+  const unsigned x = blockIdx.x, rest = x / a.heads;
+  return Item{static_cast<int>(x % a.heads), static_cast<int>(rest % a.nsplit),
               a.row_tiles - 1 - static_cast<int>(rest / a.nsplit)};
 }
 
+// Row r of a KV head: its query's number t, and its element in q and o [B,T,H,D]
+// (times D).
+struct RowAt {
+  int t;
+  int64_t row;
+};
+__device__ __forceinline__ RowAt attn_row(const AttnArgs& a, unsigned b, unsigned hk, unsigned r) {
+  const unsigned t = r / a.G;
+  return RowAt{static_cast<int>(t),
+               (static_cast<int64_t>(b) * a.T + t) * a.H + hk * a.G + (r - t * a.G)};
+}
+
+// Cache row j of a (batch, KV head), clamped to the last key.
+__device__ __forceinline__ int64_t clamp_row(int j, int L) { return min(j, L - 1); }
+
+// A decode step's norms, rotations and cache write (ember_attn_kv4_qkv).
+constexpr int kFoldRows = 8;       // new rows per call (T)
+constexpr int kMaxRopePairs = 64;  // D <= 128
+struct Fold {
+  const float* kn;    // [B, T, Hk, D] key projection
+  const float* vn;    // [B, T, Hk, D] value projection
+  const float* qn_w;  // [D] QK-Norm weights, or null (no norm)
+  const float* kn_w;
+  uint32_t* kc;  // the cache that AttnArgs reads
+  float* kp;
+  uint32_t* vc;
+  float* vp;
+  float eps;
+  float freqs[kMaxRopePairs];
+};
+
+// A query row's D/4 values per lane (dims g D/4 ..): RMSNorm, then the
+// rotation of the pairs (c, c + D/2), whose second halves lie two lane groups on.
+template <int D>
+__device__ __forceinline__ void fold_query(float (&x)[D / 4], const Fold& f,
+                                           const float (&rot)[2][D / 2], int g) {
+  if (f.qn_w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 4; ++c) ss = fmaf(x[c], x[c], ss);
+    const float rs = 1.0f / sqrtf(sum_over_rows(ss) / static_cast<float>(D) + f.eps);
+#pragma unroll
+    for (int c = 0; c < D / 4; c += 4) {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(f.qn_w + g * (D / 4) + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[c + e] = x[c + e] * rs * w[e];
+    }
+  }
+  const bool first = g < 2;
+  const int c0 = (g & 1) * (D / 4);
+#pragma unroll
+  for (int c = 0; c < D / 4; ++c) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[c]), __float_as_uint(x[c]),
+                                                    false, false);
+    const float y = __uint_as_float(first ? r[1] : r[0]);
+    const float cs = rot[0][c0 + c], sn = rot[1][c0 + c];
+    x[c] = first ? x[c] * cs - y * sn : y * sn + x[c] * cs;
+  }
+}
+
+// The new rows p = pos + t with mine(p): keys normalised and rotated, then
+// both quantised into the cache.  D/8 lanes per row; 2 T <= 16 rows fit in one
+// pass of the block's THREADS / (D/8) groups.
+template <int D, int THREADS, typename Mine>
+__device__ __forceinline__ void fold_rows(const AttnArgs& a, const Fold& f,
+                                          const float (&rot)[kFoldRows][2][D / 2], unsigned b,
+                                          unsigned hk, int bh, Mine mine) {
+  constexpr int LPR = D / 8;
+  static_assert(THREADS / LPR >= 2 * kFoldRows, "a pass holds every new row");
+  const int w = threadIdx.x % LPR, item = threadIdx.x / LPR;
+  const int T = static_cast<int>(a.T);
+  const bool value = item >= T, live = item < 2 * T;
+  const int t = live ? (value ? item - T : item) : 0;
+  const float* src = (value ? f.vn : f.kn) +
+                     ((static_cast<int64_t>(b) * T + t) * a.Hk + hk) * D + 8 * w;
+  float x[8], y[8];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const f32x4 v = reinterpret_cast<const f32x4*>(src)[c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * c + e] = y[4 * c + e] = v[e];
+  }
+  if (f.kn_w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, kWave);
+    const float rs = 1.0f / sqrtf(ss / static_cast<float>(D) + f.eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = y[e] * rs * f.kn_w[8 * w + e];
+  }
+  const bool first = w < LPR / 2;
+  const int c0 = 8 * (w % (LPR / 2));
+  float lo = INFINITY, hi = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float z = __shfl_xor(y[e], LPR / 2, kWave);
+    const float cs = rot[t][0][c0 + e], sn = rot[t][1][c0 + e];
+    const float k = first ? y[e] * cs - z * sn : z * sn + y[e] * cs;
+    x[e] = value ? x[e] : k;
+    lo = fminf(lo, x[e]);
+    hi = fmaxf(hi, x[e]);
+    bad |= not_finite(x[e]);
+  }
+  const QuantGrid g = quant_grid<LPR, 15>(lo, hi, bad);
+  if (!live || !mine(a.pos + t)) return;
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) word |= quant_code<15>(g, x[e]) << (4 * e);
+  const int64_t row = bh * a.S + a.pos + t;
+  (value ? f.vc : f.kc)[row * LPR + w] = word;
+  if (w == 0)
+    *reinterpret_cast<float2*>((value ? f.vp : f.kp) + 2 * row) = float2{g.lo, g.step};
+}
+
 // Few query rows: a workgroup owns up to 16 NT rows of one KV head and one key
-// split; its four waves take every fourth block of 32 keys, unpack their own
+// split, whose WAVES waves take blocks of 32 keys in turn (split by split, so
+// that all splits read one stretch of the cache at a time), unpack their own
 // codes and are merged through LDS.  The next block's loads (five or so per
 // lane: K as fragments, V as 16-byte pieces that pass through LDS for their
 // transpose, one pair of parameters) are in flight during a block.
-template <int D, int NT>
-__global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
+//
+// FOLD: a decode step's raw projections.  Queries are normalised and rotated as
+// they are loaded, and the workgroup whose blocks hold the new rows quantises
+// them into the cache before it reads any of its blocks; no other workgroup
+// of that head reads them, except those of another row tile, which write the
+// same bits themselves.
+template <int D, int NT, int WAVES, bool FOLD>
+__global__ __launch_bounds__(kWave * WAVES, 8 / WAVES) void attn_kv4_narrow(AttnArgs a, Fold f) {
   constexpr int W = D / 8, S = D / 32, ND = D / 16, ROWS = 16 * NT;
+  constexpr int kThreads = kWave * WAVES, kWaves = WAVES;
   constexpr int VS = W + 4;                       // words per V row in LDS
   constexpr int VP = kBlockKeys * W / 4 / kWave;  // 16-byte pieces of V per lane
   constexpr int kStage = kBlockKeys * VS + kParams * kBlockKeys;  // per wave, words
@@ -342,17 +479,14 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
 
   const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t one = two_1024();
   const Item it = attn_item(a);
-  const int64_t hk = it.bh % a.Hk, b = it.bh / a.Hk;
-  const int G = static_cast<int>(a.H / a.Hk);
-  const int64_t R = G * a.T, r0 = static_cast<int64_t>(it.tile) * ROWS;
-  const int nr = static_cast<int>(R - r0 < ROWS ? R - r0 : ROWS);
-  const int ks = it.split * a.kps;
-  const int ke = a.L - ks < a.kps ? a.L : ks + a.kps;
-  // Keys [ks, jend) are seen by some row, [ks, jall) by every one.
-  const int64_t last = a.pos + (r0 + nr - 1) / G + 1, first = a.pos + r0 / G + 1;
-  const int jend = static_cast<int>(last < ke ? last : ke);
-  const int jall = static_cast<int>(first < ke ? first : ke);
+  const unsigned b = static_cast<unsigned>(it.bh) / a.Hk, hk = it.bh - b * a.Hk;
+  const int R = a.G * a.T, r0 = it.tile * ROWS;
+  const int nr = min(R - r0, ROWS);
+  // Keys [0, jend) are seen by some row, [0, jall) by every one.
+  const int jend = min(a.pos + static_cast<int>((r0 + nr - 1) / a.G) + 1, a.L);
+  const int jall = min(a.pos + static_cast<int>(r0 / a.G) + 1, a.L);
 
   uint32_t* vbuf = reinterpret_cast<uint32_t*>(lds) + w * kStage;
   float* par = lds + w * kStage + kBlockKeys * VS;
@@ -365,7 +499,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
   auto load = [&](int j0) {  // rows past the last key read that one again
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const int64_t row = min(j0 + 16 * kt + i, a.L - 1);
+      const int64_t row = clamp_row(j0 + 16 * kt + i, a.L);
       const uint32_t* p = kc + row * W + g * S;
       if constexpr (S == 4) {
         kw[kt] = *reinterpret_cast<const u32x4*>(p);
@@ -377,13 +511,37 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
 #pragma unroll
     for (int u = 0; u < VP; ++u) {
       const int c = lane + kWave * u;
-      const int64_t row = min(j0 + c / (W / 4), a.L - 1);
+      const int64_t row = clamp_row(j0 + c / (W / 4), a.L);
       vw[u] = *reinterpret_cast<const u32x4*>(vc + row * W + 4 * (c % (W / 4)));
     }
-    pw = pp[min(j0 + (lane & 31), a.L - 1)];
+    pw = pp[clamp_row(j0 + (lane & 31), a.L)];
   };
-  const int j_first = ks + kBlockKeys * w;
-  if (j_first < jend) load(j_first);
+  const int j_first = kBlockKeys * (it.split * kWaves + w);
+  const int j_step = kBlockKeys * kWaves * a.nsplit;
+  __shared__ float rot[FOLD ? kFoldRows : 1][2][D / 2];  // cosines and sines
+  bool owner = false;  // of new rows; the same in every wave
+  if constexpr (FOLD) {
+    auto split_of = [&](int j) { return j / (kBlockKeys * kWaves) % a.nsplit; };
+    owner = split_of(a.pos) == it.split || split_of(a.L - 1) == it.split;
+  }
+  if (!owner && j_first < jend) load(j_first);
+  if constexpr (FOLD) {
+    for (int e = threadIdx.x; e < static_cast<int>(a.T) * (D / 2); e += kThreads) {
+      const int t = e / (D / 2), c = e % (D / 2);
+      float sn, cs;
+      sincosf(static_cast<float>(a.pos + t) * f.freqs[c], &sn, &cs);
+      rot[t][0][c] = cs;
+      rot[t][1][c] = sn;
+    }
+    __syncthreads();
+    if (owner) {
+      fold_rows<D, kThreads>(a, f, rot, b, hk, it.bh, [&](int p) {
+        return p / (kBlockKeys * kWaves) % a.nsplit == it.split;
+      });
+      __syncthreads();
+      if (j_first < jend) load(j_first);
+    }
+  }
 
   QRow<D> q[NT];
   int lim[NT];  // keys j < lim are seen; rows that do not exist see all
@@ -392,21 +550,23 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = 16 * n + i;
-    const int64_t t = (r0 + r) / G, h = hk * G + (r0 + r) % G;
     const bool live = r < nr;
-    q[n].load(a.q + (live ? ((b * a.T + t) * a.H + h) * D : 0), live, g, a.qscale);
-    const int64_t c = a.pos + t + 1;
-    lim[n] = live ? static_cast<int>(c < ke ? c : ke) : 0x7fffffff;
+    const RowAt at = attn_row(a, b, hk, r0 + (live ? r : 0));
+    float x[D / 4];
+    QRow<D>::load(a.q + at.row * D, live, g, x);
+    if constexpr (FOLD) fold_query<D>(x, f, rot[at.t], g);
+    q[n].set(x, a.qscale);
+    lim[n] = live ? min(a.pos + at.t + 1, a.L) : 0x7fffffff;
 #pragma unroll
     for (int t2 = 0; t2 < ND; ++t2) acc[n][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int j0 = j_first; j0 < jend; j0 += kBlockKeys * kWaves) {
+  for (int j0 = j_first; j0 < jend; j0 += j_step) {
     half8_t kf[2][S];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int k = 0; k < S; ++k) kf[kt][k] = unpack8(kw[kt][k]);
+      for (int k = 0; k < S; ++k) kf[kt][k] = unpack8(kw[kt][k], one);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -417,19 +577,19 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
     stage_params<kBlockKeys>(par, lane & 31, lane >= 32, pw, j0 + (lane & 31) < jend);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (j0 + kBlockKeys * kWaves < jend) load(j0 + kBlockKeys * kWaves);
+    if (j0 + j_step < jend) load(j0 + j_step);
 
     half8_t ph[NT], pl[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int k = 0; k < S; ++k)
+      for (int k = 0; k < S; ++k) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          s[kt] = mfma(kf[kt][k], q[n].hi[k], s[kt]);
-          s[kt] = mfma(kf[kt][k], q[n].lo[k], s[kt]);
-        }
+        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma(kf[kt][k], q[n].hi[k], s[kt]);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma(kf[kt][k], q[n].lo[k], s[kt]);
+      }
       const int vis = lim[n] - j0 - 4 * g;
       const float alpha =
           j0 + kBlockKeys > jall
@@ -448,26 +608,26 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
       vx[e] = vbuf[(16 * (e >> 2) + 4 * g + (e & 3)) * VS + (D == 128 ? i : i >> 1)];
 #pragma unroll
     for (int half = 0; half < ND / 4; ++half) {
-      half8_t u[4];
+      half8_t u[4], vf[4];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         const uint32_t x = vx[2 * p], y = vx[2 * p + 1];
         const bool high = D == 128 ? half == 1 : (i & 1) == 1;
-        u[p] = unpack8(high ? high_halves(x, y) : low_halves(x, y));
+        u[p] = unpack8(high ? high_halves(x, y) : low_halves(x, y), one);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        half8_t vf;
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          vf[2 * p] = u[p][2 * t];
-          vf[2 * p + 1] = u[p][2 * t + 1];
+          vf[t][2 * p] = u[p][2 * t];
+          vf[t][2 * p + 1] = u[p][2 * t + 1];
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][4 * half + t] = mfma(vf, ph[n], acc[n][4 * half + t]);
-          acc[n][4 * half + t] = mfma(vf, pl[n], acc[n][4 * half + t]);
-        }
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[n][4 * half + t] = mfma(vf[t], ph[n], acc[n][4 * half + t]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[n][4 * half + t] = mfma(vf[t], pl[n], acc[n][4 * half + t]);
       }
     }
   }
@@ -507,8 +667,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
       l += sm[2 * at + 1] * e;
       o += *reinterpret_cast<const f32x4*>(so + at * OS + 4 * c4) * e;
     }
-    const int64_t t = (r0 + row) / G, h = hk * G + (r0 + row) % G;
-    const int64_t orow = (b * a.T + t) * a.H + h;
+    const int64_t orow = attn_row(a, b, hk, r0 + row).row;
     if (a.nsplit == 1) {
       *reinterpret_cast<f32x4*>(a.o + orow * D + 4 * c4) = o * (1.f / l);
     } else {
@@ -528,6 +687,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_narrow(AttnArgs a) {
 // loaded during a tile and unpacked after it.
 constexpr int kWideRows = 128;
 constexpr int kTileKeys = 64;
+constexpr int64_t kWideKeys = 256;  // a split's keys at least
 
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
@@ -538,19 +698,18 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
 
   const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t one = two_1024();
   const Item it = attn_item(a);
-  const int64_t hk = it.bh % a.Hk, b = it.bh / a.Hk;
-  const int G = static_cast<int>(a.H / a.Hk);
-  const int64_t R = G * a.T, r0 = static_cast<int64_t>(it.tile) * kWideRows;
-  const int64_t rend = R - r0 < kWideRows ? R : r0 + kWideRows;
-  const int ks = it.split * a.kps;
-  const int ke = a.L - ks < a.kps ? a.L : ks + a.kps;
-  auto clip = [&](int64_t c) { return static_cast<int>(c < ke ? c : ke); };
-  const int jend = clip(a.pos + (rend - 1) / G + 1);
+  const unsigned b = static_cast<unsigned>(it.bh) / a.Hk, hk = it.bh - b * a.Hk;
+  const int r0 = it.tile * kWideRows, rend = min(static_cast<int>(a.G * a.T), r0 + kWideRows);
+  const int ks = kTileKeys * it.split, j_step = kTileKeys * a.nsplit;
+  // How many keys row r sees.
+  auto seen = [&](int r) { return min(a.pos + static_cast<int>(r / a.G) + 1, a.L); };
+  const int jend = seen(rend - 1);
   // This wave's rows, and the keys that some and all of them see.
-  const int64_t wr0 = r0 + 32 * w, wrend = rend - wr0 < 32 ? rend : wr0 + 32;
-  const int wend = wr0 < rend ? clip(a.pos + (wrend - 1) / G + 1) : ks;
-  const int wall = wr0 < rend ? clip(a.pos + wr0 / G + 1) : ks;
+  const int wr0 = r0 + 32 * w;
+  const int wend = wr0 < rend ? seen(min(wr0 + 32, rend) - 1) : 0;
+  const int wall = wr0 < rend ? seen(wr0) : 0;
 
   const uint32_t* kc = a.kc + it.bh * a.S * W;
   const uint32_t* vc = a.vc + it.bh * a.S * W;
@@ -560,7 +719,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
   uint32_t vw[4];
   float2 pw = {0.f, 0.f};
   auto load = [&](int j0) {  // rows past the last key read that one again
-    const int64_t row = min(j0 + 16 * w + i, a.L - 1);
+    const int64_t row = clamp_row(j0 + 16 * w + i, a.L);
     const uint32_t* p = kc + row * W + g * S;
     if constexpr (S == 4) {
       kw = *reinterpret_cast<const u32x4*>(p);
@@ -570,19 +729,19 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t vrow = min(j0 + 16 * w + 4 * g + e, a.L - 1);
+      const int64_t vrow = clamp_row(j0 + 16 * w + 4 * g + e, a.L);
       vw[e] = vc[vrow * W + (D == 128 ? i : i >> 1)];
     }
-    if (w < 2) pw = pp[min(j0 + lane, a.L - 1)];
+    if (w < 2) pw = pp[clamp_row(j0 + lane, a.L)];
   };
   auto stage = [&](int buf, int j0) {
 #pragma unroll
-    for (int k = 0; k < S; ++k) kfrag[buf][w][k][lane] = unpack8(kw[k]);
+    for (int k = 0; k < S; ++k) kfrag[buf][w][k][lane] = unpack8(kw[k], one);
 #pragma unroll
     for (int half = 0; half < ND / 4; ++half) {
       const bool high = D == 128 ? half == 1 : (i & 1) == 1;
-      const half8_t x = unpack8(high ? high_halves(vw[0], vw[1]) : low_halves(vw[0], vw[1]));
-      const half8_t y = unpack8(high ? high_halves(vw[2], vw[3]) : low_halves(vw[2], vw[3]));
+      const half8_t x = unpack8(high ? high_halves(vw[0], vw[1]) : low_halves(vw[0], vw[1]), one);
+      const half8_t y = unpack8(high ? high_halves(vw[2], vw[3]) : low_halves(vw[2], vw[3]), one);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
         reinterpret_cast<half4_t*>(&vfrag[buf][w >> 1][4 * half + t][lane])[w & 1] =
@@ -598,11 +757,13 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
   f32x4 acc[NT][ND];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int64_t r = wr0 + 16 * n + i;
-    const int64_t t = r / G, h = hk * G + r % G;
+    const int r = wr0 + 16 * n + i;
     const bool live = r < rend;
-    q[n].load(a.q + (live ? ((b * a.T + t) * a.H + h) * D : 0), live, g, a.qscale);
-    lim[n] = live ? clip(a.pos + t + 1) : 0x7fffffff;
+    const RowAt at = attn_row(a, b, hk, live ? r : r0);
+    float x[D / 4];
+    QRow<D>::load(a.q + at.row * D, live, g, x);
+    q[n].set(x, a.qscale);
+    lim[n] = live ? min(a.pos + at.t + 1, a.L) : 0x7fffffff;
 #pragma unroll
     for (int t2 = 0; t2 < ND; ++t2) acc[n][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -610,9 +771,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
   __syncthreads();
 
   int buf = 0;
-  for (int j0 = ks; j0 < jend; j0 += kTileKeys, buf ^= 1) {
-    const bool more = j0 + kTileKeys < jend;
-    if (more) load(j0 + kTileKeys);
+  for (int j0 = ks; j0 < jend; j0 += j_step, buf ^= 1) {
+    const bool more = j0 + j_step < jend;
+    if (more) load(j0 + j_step);
 #pragma unroll
     for (int u = 0; u < kTileKeys / 32; ++u) {
       const int jb = j0 + 32 * u;
@@ -658,17 +819,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
         }
       }
     }
-    if (more) stage(buf ^ 1, j0 + kTileKeys);
+    if (more) stage(buf ^ 1, j0 + j_step);
     __syncthreads();
   }
 
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float l = sum_over_rows(st[n].l), olo = sum_over_rows(st[n].olo);
-    const int64_t r = wr0 + 16 * n + i;
+    const int r = wr0 + 16 * n + i;
     if (r >= rend) continue;
-    const int64_t t = r / G, h = hk * G + r % G;
-    const int64_t orow = (b * a.T + t) * a.H + h;
+    const int64_t orow = attn_row(a, b, hk, r).row;
     const float mul = a.nsplit == 1 ? 1.f / l : 1.f;
     float* out = a.nsplit == 1 ? a.o + orow * D
                                : a.part_o + (orow * a.nsplit + it.split) * D;
@@ -687,84 +847,92 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
   }
 }
 
-// Merges a row's splits in split order: a wave per row.  The splits' weights
-// are formed a lane each and kept in LDS, so the loop over splits only streams
-// partial rows.
-template <int D>
+// Merges a row's splits in a fixed order.  PARTS groups of D/4 lanes take every
+// PARTS-th split of a row each, four at a time, and are then added in order:
+// a wave per row (PARTS = 256 / D) where splits are few, a block per row (1024 / D)
+// where they are many (64 splits of 16 rows: 3.4 -> 2.6 us).
+template <int D, int PARTS>
 __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __restrict__ part_o,
                                                              const float* __restrict__ part_ml,
-                                                             float* __restrict__ o, int64_t rows,
+                                                             float* __restrict__ o, int rows,
                                                              int nsplit) {
-  constexpr int PER = D / kWave;
-  __shared__ float s_e[kWaves][kMaxSplits];
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + w;
-  if (row >= rows) return;  // whole waves leave; no block barrier follows
-  const float* ml = part_ml + row * nsplit * 2;
+  constexpr int LANES = D / 4, PER_ROW = PARTS * LANES, RPB = kThreads / PER_ROW;
+  __shared__ f32x4 s_o[kThreads];
+  __shared__ float s_l[kThreads];
+  __shared__ float s_m[kThreads / kWave];
+  const int c4 = threadIdx.x % LANES, part = threadIdx.x / LANES % PARTS;
+  const int row = blockIdx.x * RPB + threadIdx.x / PER_ROW;
+  const bool live = row < rows;
+  const float* ml = part_ml + static_cast<int64_t>(live ? row : 0) * nsplit * 2;
+  const float* po = part_o + static_cast<int64_t>(live ? row : 0) * nsplit * D + 4 * c4;
+  const int own = threadIdx.x % PER_ROW;
   float M = -INFINITY;
-  for (int s = lane; s < nsplit; s += kWave) M = fmaxf(M, ml[2 * s]);
+  for (int s = own; s < nsplit; s += PER_ROW) M = fmaxf(M, ml[2 * s]);
   M = wave_max(M);
+  if constexpr (PER_ROW > kWave) {
+    if (threadIdx.x % kWave == 0) s_m[threadIdx.x / kWave] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) M = fmaxf(M, s_m[w]);
+  }
   float l = 0.f;
-  for (int s = lane; s < nsplit; s += kWave) {
-    const float e = merge_weight(ml[2 * s], ml[2 * s + 1], M);
-    s_e[w][s] = e;
-    l += ml[2 * s + 1] * e;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = part; s < nsplit; s += PARTS) {
+    const float ls = ml[2 * s + 1], e = merge_weight(ml[2 * s], ls, M);
+    l += ls * e;
+    acc += *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(s) * D) * e;
   }
-  l = wave_sum(l);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  float acc[PER] = {};
-  const float* po = part_o + row * nsplit * D + lane;
-  int s = 0;
-  for (; s + 8 <= nsplit; s += 8) {
-    float x[8][PER];
+  s_o[threadIdx.x] = acc;
+  s_l[threadIdx.x] = l;
+  __syncthreads();
+  if (part == 0 && live) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int p = 0; p < PER; ++p) x[u][p] = po[(s + u) * D + p * kWave];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int p = 0; p < PER; ++p) acc[p] += x[u][p] * s_e[w][s + u];
+    for (int p = 1; p < PARTS; ++p) {
+      acc += s_o[threadIdx.x + p * LANES];
+      l += s_l[threadIdx.x + p * LANES];
+    }
+    *reinterpret_cast<f32x4*>(o + static_cast<int64_t>(row) * D + 4 * c4) = acc * (1.f / l);
   }
-  for (; s < nsplit; ++s)
-#pragma unroll
-    for (int p = 0; p < PER; ++p) acc[p] += po[s * D + p * kWave] * s_e[w][s];
-  const float inv = 1.0f / l;
-#pragma unroll
-  for (int p = 0; p < PER; ++p) o[row * D + p * kWave + lane] = acc[p] * inv;
 }
 
-// How a call is laid out.  Up to 16 rows a KV head (a decode step) one query
-// tile, up to kNarrowRows two, beyond that the shared tiles of 128 rows.  Keys
-// are split until there are kTargetBlocks workgroups, each with at least one
-// block of 32 keys per wave (narrow) or kWideKeys keys (wide).
-constexpr int64_t kNarrowRows = 64;
-constexpr int64_t kTargetBlocks = 512;
-constexpr int64_t kNarrowKeys = kBlockKeys * kWaves;
-constexpr int64_t kWideKeys = 512;
+// How a call is laid out, R = rows of a KV head (us for 8 KV heads of D = 128 on
+// an MI355X).
+//  - R <= 16, a decode step: one query tile.  Up to kOneKeys keys, or where every
+//    CU has a head of its own, one workgroup of eight waves per head and no second
+//    launch (257 keys 5.2 against 6.4 in splits of four waves, 512 keys 7.6 and
+//    7.3, 1024 keys 8.6 and 7.3; 256 heads of 4000 keys 33.9 and 36.0); else splits.
+//  - R <= kNarrowRows: two query tiles; beyond, the shared tiles of 128 rows.
+//  - Splits: a workgroup for each CU, two where that leaves kLongKeys keys or more
+//    to each (130001 keys 36 against 42 with one; 4096 keys and 128 rows, where
+//    the partial results weigh more, 23 against 19), and 32 keys a wave at least.
+constexpr int64_t kCus = 256;
+constexpr int64_t kOneKeys = 512;
+constexpr int64_t kNarrowRows = 256;
+constexpr int64_t kLongKeys = 1024;
+constexpr int kOneWaves = 8;
+
+enum Variant { kOne, kTile, kTwoTiles, kWide };
 
 struct Plan {
-  int variant;  // 1, 2: narrow with that many query tiles; 0: wide
+  Variant variant;
   int nsplit;
-  int64_t row_tiles, kps;
+  int64_t row_tiles;
 };
 
 Plan attn_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t L) {
-  const int64_t R = H / Hk * T;
-  Plan p{};
-  p.variant = R <= 16 ? 1 : R <= kNarrowRows ? 2 : 0;
-  const int64_t rows = p.variant ? 16 * p.variant : kWideRows;
-  const int64_t unit = p.variant ? kNarrowKeys : kWideKeys;
-  p.row_tiles = (R + rows - 1) / rows;
-  const int64_t items = B * Hk * p.row_tiles;
-  int64_t want = (kTargetBlocks + items - 1) / items;
+  const int64_t R = H / Hk * T, heads = B * Hk;
+  if (R <= 16 && (L <= kOneKeys || heads >= kCus)) return Plan{kOne, 1, 1};
+  const Variant variant = R <= 16 ? kTile : R <= kNarrowRows ? kTwoTiles : kWide;
+  const int64_t rows = variant == kTile ? 16 : variant == kTwoTiles ? 32 : kWideRows;
+  const int64_t unit = variant == kWide ? kWideKeys : kBlockKeys * kWaves;
+  const int64_t row_tiles = (R + rows - 1) / rows, items = heads * row_tiles;
+  int64_t want = (kCus + items - 1) / items;
+  if (L / want >= kLongKeys) want = (2 * kCus + items - 1) / items;
   const int64_t units = (L + unit - 1) / unit;
   if (want > units) want = units;
   if (want > kMaxSplits) want = kMaxSplits;
-  p.kps = (units + want - 1) / want * unit;
-  p.nsplit = static_cast<int>((L + p.kps - 1) / p.kps);
-  return p;
+  return Plan{variant, static_cast<int>(want), row_tiles};
 }
 
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
@@ -819,6 +987,75 @@ extern "C" size_t ember_attn_kv4_workspace_bytes(int64_t B, int64_t T, int64_t H
   return static_cast<size_t>(B * T * H) * p.nsplit * (D + 2) * sizeof(float);
 }
 
+namespace {
+
+// Shared by ember_attn_kv4 and ember_attn_kv4_qkv (fold != null).
+int run_attn(const float* q, const uint32_t* kc, const float* kp, const uint32_t* vc,
+             const float* vp, float* o, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
+             int64_t L, int64_t pos, int64_t S, float scale, void* workspace,
+             size_t workspace_bytes, const Fold* fold, hipStream_t st) {
+  const Plan p = attn_plan(B, T, H, Hk, L);
+  const int64_t blocks = B * Hk * p.row_tiles * p.nsplit;
+  const int64_t rows = B * T * H;
+  if (blocks > 0x7fffffff || rows > 0x7fffffff) return EMBER_EINVAL;
+  const size_t need = ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, L);
+  if (need && (!workspace || workspace_bytes < need)) return EMBER_EWORKSPACE;
+  if (need && !aligned16(workspace)) return EMBER_EALIGN;
+  AttnArgs a{};
+  a.q = q;
+  a.kc = kc;
+  a.kp = kp;
+  a.vc = vc;
+  a.vp = vp;
+  a.o = o;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = need ? a.part_o + rows * p.nsplit * D : nullptr;
+  a.S = S;
+  a.heads = static_cast<unsigned>(B * Hk);
+  a.T = static_cast<unsigned>(T);
+  a.H = static_cast<unsigned>(H);
+  a.Hk = static_cast<unsigned>(Hk);
+  a.G = static_cast<unsigned>(H / Hk);
+  a.pos = static_cast<int>(pos);
+  a.L = static_cast<int>(L);
+  a.nsplit = p.nsplit;
+  a.row_tiles = static_cast<int>(p.row_tiles);
+  a.qscale = scale * 1.4426950408889634f;
+  auto launch = [&](auto d, auto folded) {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool FOLD = decltype(folded)::value;
+    const Fold f = fold ? *fold : Fold{};
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.variant == kOne)
+      attn_kv4_narrow<DD, 1, kOneWaves, FOLD><<<grid, kWave * kOneWaves, 0, st>>>(a, f);
+    else if (p.variant == kTile)
+      attn_kv4_narrow<DD, 1, kWaves, FOLD><<<grid, kThreads, 0, st>>>(a, f);
+    else if (p.variant == kTwoTiles)
+      attn_kv4_narrow<DD, 2, kWaves, FOLD><<<grid, kThreads, 0, st>>>(a, f);
+    else if (!FOLD)
+      attn_kv4_wide<DD><<<grid, kThreads, 0, st>>>(a);
+    else
+      return static_cast<int>(EMBER_EINVAL);
+    const int rc = launch_status();
+    if (rc || p.nsplit == 1) return rc;
+    constexpr int kWaveParts = 256 / DD, kBlockParts = 1024 / DD;
+    if (p.nsplit > 2 * kWaveParts)
+      attn_kv4_combine<DD, kBlockParts><<<static_cast<unsigned>(rows), kThreads, 0, st>>>(
+          a.part_o, a.part_ml, o, static_cast<int>(rows), p.nsplit);
+    else
+      attn_kv4_combine<DD, kWaveParts>
+          <<<static_cast<unsigned>((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(
+              a.part_o, a.part_ml, o, static_cast<int>(rows), p.nsplit);
+    return launch_status();
+  };
+  using D128 = std::integral_constant<int, 128>;
+  using D64 = std::integral_constant<int, 64>;
+  if (fold) return D == 128 ? launch(D128{}, std::true_type{}) : launch(D64{}, std::true_type{});
+  return D == 128 ? launch(D128{}, std::false_type{}) : launch(D64{}, std::false_type{});
+}
+
+}  // namespace
+
 extern "C" int ember_attn_kv4(const float* q, const uint32_t* k_codes, const float* k_params,
                               const uint32_t* v_codes, const float* v_params, float* o, int64_t B,
                               int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t L, int64_t pos,
@@ -832,49 +1069,39 @@ extern "C" int ember_attn_kv4(const float* q, const uint32_t* k_codes, const flo
   if (!aligned16(q) || !aligned16(o) || !aligned16(k_codes) || !aligned16(v_codes) ||
       !aligned8(k_params) || !aligned8(v_params))
     return EMBER_EALIGN;
-  const Plan p = attn_plan(B, T, H, Hk, L);
-  const int64_t blocks = B * Hk * p.row_tiles * p.nsplit;
-  const int64_t rows = B * T * H;
-  if (blocks > 0x7fffffff || rows > 0x7fffffff || p.kps > 0x7fffffff) return EMBER_EINVAL;
-  const size_t need = ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, L);
-  if (need && (!workspace || workspace_bytes < need)) return EMBER_EWORKSPACE;
-  if (need && !aligned16(workspace)) return EMBER_EALIGN;
-  AttnArgs a{};
-  a.q = q;
-  a.kc = k_codes;
-  a.kp = k_params;
-  a.vc = v_codes;
-  a.vp = v_params;
-  a.o = o;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = need ? a.part_o + rows * p.nsplit * D : nullptr;
-  a.T = T;
-  a.H = H;
-  a.Hk = Hk;
-  a.pos = pos;
-  a.S = S;
-  a.heads = B * Hk;
-  a.L = static_cast<int>(L);
-  a.kps = static_cast<int>(p.kps);
-  a.nsplit = p.nsplit;
-  a.row_tiles = static_cast<int>(p.row_tiles);
-  a.qscale = scale * 1.4426950408889634f;
-  hipStream_t st = as_stream(s);
-  auto launch = [&](auto d) {
-    constexpr int DD = decltype(d)::value;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (p.variant == 1)
-      attn_kv4_narrow<DD, 1><<<grid, kThreads, 0, st>>>(a);
-    else if (p.variant == 2)
-      attn_kv4_narrow<DD, 2><<<grid, kThreads, 0, st>>>(a);
-    else
-      attn_kv4_wide<DD><<<grid, kThreads, 0, st>>>(a);
-    const int rc = launch_status();
-    if (rc || p.nsplit == 1) return rc;
-    attn_kv4_combine<DD><<<static_cast<unsigned>((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(
-        a.part_o, a.part_ml, o, rows, p.nsplit);
-    return launch_status();
-  };
-  return D == 128 ? launch(std::integral_constant<int, 128>{})
-                  : launch(std::integral_constant<int, 64>{});
+  return run_attn(q, k_codes, k_params, v_codes, v_params, o, B, T, H, Hk, D, L, pos, S, scale,
+                  workspace, workspace_bytes, nullptr, as_stream(s));
+}
+
+extern "C" int ember_attn_kv4_qkv(const float* q, const float* k, const float* v, int64_t B,
+                                  int64_t T, int64_t H, int64_t Hk, int64_t D,
+                                  const float* q_norm_w, const float* k_norm_w, float eps,
+                                  const float* freqs_host, int64_t pos, uint32_t* k_codes,
+                                  float* k_params, uint32_t* v_codes, float* v_params, int64_t S,
+                                  float scale, float* o, void* workspace, size_t workspace_bytes,
+                                  ember_stream_t s) {
+  if (B < 0 || T < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || pos < 0 || !freqs_host)
+    return EMBER_EINVAL;
+  if ((D != 64 && D != 128) || T > kFoldRows || H / Hk > kNarrowRows / kFoldRows)
+    return EMBER_EINVAL;
+  if (S > kMaxRows || T > S || pos > S - T) return EMBER_EINVAL;
+  if (B == 0 || T == 0) return EMBER_OK;
+  if (!q || !k || !v || !o || !k_codes || !k_params || !v_codes || !v_params) return EMBER_EINVAL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(k_codes) ||
+      !aligned16(v_codes) || !aligned8(k_params) || !aligned8(v_params) ||
+      (q_norm_w && !aligned16(q_norm_w)) || (k_norm_w && !aligned16(k_norm_w)))
+    return EMBER_EALIGN;
+  Fold f{};
+  f.kn = k;
+  f.vn = v;
+  f.qn_w = q_norm_w;
+  f.kn_w = k_norm_w;
+  f.kc = k_codes;
+  f.kp = k_params;
+  f.vc = v_codes;
+  f.vp = v_params;
+  f.eps = eps;
+  for (int64_t i = 0; i < D / 2; ++i) f.freqs[i] = freqs_host[i];
+  return run_attn(q, k_codes, k_params, v_codes, v_params, o, B, T, H, Hk, D, pos + T, pos, S,
+                  scale, workspace, workspace_bytes, &f, as_stream(s));
 }

@@ -119,6 +119,10 @@ _SIGS = {
     "ctd_set_attn_keep_scores": (i32, [i32]),
     "ctd_trainer_generate": (i32, [vp, lptr, i64, i32, f32, i32, f32, u64, i64, lptr,
                                    C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "ctd_trainer_set_checkpoint_bits": (i32, [vp, i32]),
+    "ctd_kvcache_create_bits": (i32, [vp, i64, i64, i32, C.POINTER(vp)]),
+    "ctd_trainer_generate_bits": (i32, [vp, lptr, i64, i32, f32, i32, f32, u64, i64, i32, lptr,
+                                        C.POINTER(C.c_double), C.POINTER(C.c_double)]),
 }
 
 
@@ -260,6 +264,10 @@ class Trainer:
         _ck(rc, "get_grad")
         return out
 
+    def set_checkpoint_bits(self, bits):
+        """How a checkpointed block's input is held: 32 bits (as it is) or 8."""
+        _ck(lib().ctd_trainer_set_checkpoint_bits(self.h, bits), "set_checkpoint_bits")
+
     def set_checkpointing(self, on):
         _ck(lib().ctd_trainer_set_checkpointing(self.h, int(on)), "set_checkpointing")
 
@@ -370,20 +378,20 @@ class Trainer:
         return len(self.names)
 
     def generate(self, prompt, max_new, temperature=0.0, top_k=0, top_p=0.0, seed=0,
-                 max_seq=None):
+                 max_seq=None, kv_bits=32):
         """ctd_generate's loop (batch 1): (tokens, prefill_ms, decode_ms)."""
         prompt = np.ascontiguousarray(prompt, dtype=np.int64)
         toks = np.zeros(max_new, np.int64)
         pf, dc = C.c_double(), C.c_double()
-        _ck(lib().ctd_trainer_generate(self.h, prompt.ctypes.data_as(lptr), prompt.size, max_new,
-                                       temperature, top_k, top_p, seed,
-                                       max_seq or prompt.size + max_new,
-                                       toks.ctypes.data_as(lptr), C.byref(pf), C.byref(dc)),
+        _ck(lib().ctd_trainer_generate_bits(self.h, prompt.ctypes.data_as(lptr), prompt.size,
+                                            max_new, temperature, top_k, top_p, seed,
+                                            max_seq or prompt.size + max_new, kv_bits,
+                                            toks.ctypes.data_as(lptr), C.byref(pf), C.byref(dc)),
             "generate")
         return toks, pf.value, dc.value
 
-    def kv_cache(self, batch, max_seq):
-        return KVCache(self, batch, max_seq)
+    def kv_cache(self, batch, max_seq, bits=32):
+        return KVCache(self, batch, max_seq, bits)
 
     def forward(self, ids, cache=None, position_start=0, last_only=False):
         """Model::forward (or forward_last_logits) of host int64 ids [B,T] -> logits."""
@@ -398,11 +406,12 @@ class Trainer:
 
 
 class KVCache:
-    """nn::KVCache for a trainer's model (zero-filled, batch x max_seq rows)."""
+    """nn::KVCache for a trainer's model (zero-filled, batch x max_seq rows of 32 or 4 bits)."""
 
-    def __init__(self, tr: Trainer, batch, max_seq):
+    def __init__(self, tr: Trainer, batch, max_seq, bits=32):
+        self.h = None
         h = vp()
-        _ck(lib().ctd_kvcache_create(tr.h, batch, max_seq, C.byref(h)), "kv_cache")
+        _ck(lib().ctd_kvcache_create_bits(tr.h, batch, max_seq, bits, C.byref(h)), "kv_cache")
         self.h = h
 
     @property

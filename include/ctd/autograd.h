@@ -8,6 +8,8 @@
 
 #include "ctd/tensor.h"
 
+namespace ctd::ops { struct NormValues; }
+
 namespace ctd::autograd {
 
 class Node;
@@ -82,5 +84,17 @@ void accumulate_inplace(Tensor& dst, const Tensor& src);
 // Runs fn(input) without recording the tape and re-runs it with autograd
 // during backward.  fn must be a pure function of input and parameter leaves.
 Tensor checkpoint(std::function<Tensor(const Tensor&)> fn, const Tensor& input);
+
+// checkpoint() that holds its input in 8 bits (ops/quant.h) until the backward
+// pass, a quarter of the memory.  The forward pass runs fn on the input itself;
+// the backward pass re-runs it on the restored input, so the gradients are
+// fn's at a point that is off by at most half a step per value.  input fp32.
+// Added in this build.
+Tensor checkpoint_q8(std::function<Tensor(const Tensor&)> fn, const Tensor& input);
+// The same for an fn that begins with RMSNorm(input; norm_weight, eps): in the
+// backward pass it also gets that norm's values (ops::rms_norm_from), formed as
+// the rows are restored; in the forward pass a null pointer.
+Tensor checkpoint_q8(std::function<Tensor(const Tensor&, const ops::NormValues*)> fn,
+                     const Tensor& input, const Tensor& norm_weight, float norm_eps);
 
 }  // namespace ctd::autograd

@@ -7,7 +7,8 @@
 //    "max_new_tokens": 64, "max_seq_len": 2048,
 //    "temperature": 1.0, "top_k": 0, "top_p": 0.0, "seed": 0,
 //    "eos_ids": [int...],
-//    "thinking_token_budget": 0, "think_open_ids": [...], "think_close_ids": [...]}
+//    "thinking_token_budget": 0, "think_open_ids": [...], "think_close_ids": [...],
+//    "kv_bits": 32}                     32 or 4 (added in this build)
 // Reply: one JSON line per generated token {"token":id}, then
 //   {"done":true,"generated_tokens":n,"reason":"max_tokens"|"eos"|"max_seq_len"},
 // or {"done":true,"reason":"empty_prompt"|"max_seq_len"} before any token, or
@@ -33,6 +34,7 @@ struct Request {
   int thinking_token_budget = 0;
   std::vector<int64_t> think_open_ids;
   std::vector<int64_t> think_close_ids;
+  int kv_bits = 32;  // 4: a KV cache held in 4 bits (nn::KVCache::allocate)
 };
 
 // Parses a request; throws std::runtime_error on bad JSON or field types.

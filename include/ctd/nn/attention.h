@@ -64,7 +64,9 @@ struct Attention {
 
   // Inference forward (no autograd).  Positions start at position_start.  With
   // kv, this call's K/V go to cache rows [position_start, position_start+T)
-  // and the queries attend over rows [0, position_start+T).
+  // and the queries attend over rows [0, position_start+T).  With a 4-bit
+  // cache they attend over what it holds, their own rows included, so that a
+  // result does not depend on how the tokens were split into calls.
   Tensor forward(const Tensor& x, KVLayer* kv = nullptr, int position_start = 0) const {
     return o_proj.forward(forward_context(x, kv, position_start));
   }
@@ -89,17 +91,26 @@ struct Attention {
     }
     const float scale = 1.0f / std::sqrt(static_cast<float>(D));
     Tensor A;
-    if (kv != nullptr) {
+    const bool kv4 = kv != nullptr && kv->kv4();
+    if (kv4) {
+      ops::write_kv4_inplace(kv->k, kv->k_params, kv->v, kv->v_params, K, V, position_start);
+    } else if (kv != nullptr) {
       ops::write_kv_inplace(kv->k, K, position_start);
       ops::write_kv_inplace(kv->v, V, position_start);
     }
     if (!fused_head_dim(D)) {
       const int L = kv ? position_start + static_cast<int>(T) : static_cast<int>(T);
-      Tensor Kr = kv ? ops::read_kv_expanded(kv->k, L, group())
-                     : ops::permute(ops::repeat_kv_heads(K, group()), {0, 2, 1, 3});
-      Tensor Vr = kv ? ops::read_kv_expanded(kv->v, L, group())
-                     : ops::permute(ops::repeat_kv_heads(V, group()), {0, 2, 1, 3});
+      auto rows = [&](const Tensor& fresh, const Tensor* cache, const Tensor* params) {
+        if (kv4) return ops::read_kv4_expanded(*cache, *params, L, group());
+        if (kv) return ops::read_kv_expanded(*cache, L, group());
+        return ops::permute(ops::repeat_kv_heads(fresh, group()), {0, 2, 1, 3});
+      };
+      Tensor Kr = rows(K, kv ? &kv->k : nullptr, kv ? &kv->k_params : nullptr);
+      Tensor Vr = rows(V, kv ? &kv->v : nullptr, kv ? &kv->v_params : nullptr);
       A = attention_chain(Q, Kr, Vr, position_start, scale);
+    } else if (kv4) {
+      A = ops::cached_attention_kv4(Q, kv->k, kv->k_params, kv->v, kv->v_params,
+                                    position_start + T, position_start, scale);
     } else if (position_start == 0) {
       // Prefill: every visible key is one of these T, so the training kernel
       // (MFMA tiles) runs on the fresh projections.

@@ -51,6 +51,10 @@ struct Model {
   std::vector<TransformerBlock> layers;
   RMSNorm norm;
   bool gradient_checkpointing = false;
+  // With gradient_checkpointing: how a block's input is held until the backward
+  // pass, in 32 bits (as it is) or in 8 (autograd::checkpoint_q8: a quarter of
+  // the checkpoints' memory, gradients at the restored inputs).
+  int checkpoint_bits = 32;
   // Called with the layer index when the backward pass re-runs a checkpointed
   // layer's forward, before the re-run (never during the forward pass itself).
   // A trainer uses it to start work that should overlap the end of the

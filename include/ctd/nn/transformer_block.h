@@ -23,7 +23,8 @@ struct TransformerBlock {
   Tensor forward(const Tensor& x, KVLayer* kv = nullptr, int position_start = 0) const {
     autograd::NoGradGuard ng;
     if (kv != nullptr && x.dim() == 3 && x.shape()[0] * x.shape()[1] <= ops::kDecodeMaxRows &&
-        Attention::fused_head_dim(self_attn.head_dim))
+        Attention::fused_head_dim(self_attn.head_dim) &&
+        (!kv->kv4() || self_attn.group() <= ops::kDecodeKv4MaxGroup))
       return decode_step(x, *kv, position_start);
     Tensor h1 = input_layernorm.forward(x);
     Tensor h = self_attn.o_proj.forward_add(self_attn.forward_context(h1, kv, position_start), x);
@@ -37,10 +38,16 @@ struct TransformerBlock {
     const int H = at.num_heads, Hk = at.num_kv_heads, D = at.head_dim;
     auto qkv = ops::decode_linear(x, input_layernorm.weight, input_layernorm.eps,
                                   {at.q_proj.weight, at.k_proj.weight, at.v_proj.weight});
-    Tensor a = ops::decode_qkv_attention(qkv[0], qkv[1], qkv[2], H, Hk, D, at.q_norm.weight,
-                                         at.k_norm.weight, at.q_norm.eps, at.rope_theta,
-                                         at.rope_scaling, position_start, kv.k, kv.v,
-                                         1.0f / std::sqrt(static_cast<float>(D)));
+    const float scale = 1.0f / std::sqrt(static_cast<float>(D));
+    Tensor a =
+        kv.kv4()
+            ? ops::decode_qkv_attention_kv4(qkv[0], qkv[1], qkv[2], H, Hk, D, at.q_norm.weight,
+                                            at.k_norm.weight, at.q_norm.eps, at.rope_theta,
+                                            at.rope_scaling, position_start, kv.k, kv.k_params,
+                                            kv.v, kv.v_params, scale)
+            : ops::decode_qkv_attention(qkv[0], qkv[1], qkv[2], H, Hk, D, at.q_norm.weight,
+                                        at.k_norm.weight, at.q_norm.eps, at.rope_theta,
+                                        at.rope_scaling, position_start, kv.k, kv.v, scale);
     Tensor h = ops::decode_linear(a.reshape({B, T, static_cast<int64_t>(H) * D}), Tensor{}, 0.0f,
                                   {at.o_proj.weight}, {x})[0];
     Tensor m = ops::decode_gate_up(h, post_attention_layernorm.weight,
@@ -65,8 +72,11 @@ struct TransformerBlock {
   // copy_to_host() throw).  Its gradients are forward_train's, kernel for
   // kernel.  The checkpointed forward already computed the real output: it is
   // the next block's saved input.
-  Tensor forward_train_for_backward(const Tensor& x) const {
-    Tensor h1 = input_layernorm.forward(x);
+  // normed: input_layernorm's values at x where they are known
+  // (autograd::checkpoint_q8 restores them with x).
+  Tensor forward_train_for_backward(const Tensor& x,
+                                    const ops::NormValues* normed = nullptr) const {
+    Tensor h1 = normed ? input_layernorm.forward_from(x, *normed) : input_layernorm.forward(x);
     Tensor h = self_attn.o_proj.forward_add(self_attn.forward_train_context(h1), x);
     Tensor h2 = post_attention_layernorm.forward(h);
     Tensor m = mlp.down_proj.forward_graph_only(mlp.activation(h2), h);

@@ -47,7 +47,12 @@ Tensor causal_attention_impl(const Tensor& q, const Tensor& k, const Tensor& v, 
 // include/ctd/nn/attention.h:66-91).  -> o [B,T,H,D].
 Tensor cached_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
                         int64_t valid_len, int position_start, float scale);
-// The same over k/v [B,T,Hk,D] projections (no cache; valid_len = T).
+// cached_attention over a cache held in 4 bits (ops/kv_cache.h), for any number
+// of queries.  Added in this build.
+Tensor cached_attention_kv4(const Tensor& q, const Tensor& k_codes, const Tensor& k_params,
+                            const Tensor& v_codes, const Tensor& v_params, int64_t valid_len,
+                            int position_start, float scale);
+// cached_attention over k/v [B,T,Hk,D] projections (no cache; valid_len = T).
 Tensor offset_attention(const Tensor& q, const Tensor& k, const Tensor& v, int position_start,
                         float scale);
 

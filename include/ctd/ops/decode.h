@@ -42,4 +42,14 @@ Tensor decode_qkv_attention(const Tensor& q, const Tensor& k, const Tensor& v, i
                             const RopeScaling& scaling, int position_start, Tensor& k_cache,
                             Tensor& v_cache, float scale);
 
+// decode_qkv_attention over a cache held in 4 bits (ops/kv_cache.h): the new
+// rows are quantised into it in the attention's launch.  num_heads /
+// num_kv_heads at most kDecodeKv4MaxGroup.
+constexpr int kDecodeKv4MaxGroup = 32;
+Tensor decode_qkv_attention_kv4(const Tensor& q, const Tensor& k, const Tensor& v, int num_heads,
+                                int num_kv_heads, int head_dim, const Tensor& q_norm_w,
+                                const Tensor& k_norm_w, float eps, float theta,
+                                const RopeScaling& scaling, int position_start, Tensor& k_codes,
+                                Tensor& k_params, Tensor& v_codes, Tensor& v_params, float scale);
+
 }  // namespace ctd::ops

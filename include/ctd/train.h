@@ -42,6 +42,7 @@ struct Config {
   uint64_t seed = 42;
   bool offload_optimizer = false;
   bool gradient_checkpointing = false;
+  int checkpoint_bits = 32;  // 8: Model::checkpoint_bits (added in this build)
   // Optional "model" object (not in the reference, which only autodetects its
   // presets from the embedding shape): LlamaConfig fields by name, for shapes
   // autodetection does not know, e.g. small test models.

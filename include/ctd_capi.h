@@ -84,6 +84,10 @@ int ctd_trainer_get_param(ctd_trainer_t t, int64_t i, float* host, int64_t numel
 int ctd_trainer_get_grad(ctd_trainer_t t, int64_t i, float* host, int64_t numel);
 
 int ctd_trainer_set_checkpointing(ctd_trainer_t t, int32_t on);
+/* How a checkpointed block's input is held until the backward pass: 32 bits (the
+ * default: as it is) or 8 (Model::checkpoint_bits).  Also holds for
+ * ctd_trainer_block_step's checkpoint. */
+int ctd_trainer_set_checkpoint_bits(ctd_trainer_t t, int32_t bits);
 /* Batch: ids/targets int64 [B,T], mask fp32 [B,T] (NULL = all ones), host memory. */
 int ctd_trainer_set_batch(ctd_trainer_t t, const int64_t* ids, const int64_t* targets,
                           const float* mask, int64_t B, int64_t T);
@@ -204,6 +208,9 @@ int ctd_train_event_json(int32_t step, float loss, float lr, float grad_norm,
 typedef void* ctd_kvcache_t;
 /* A zero-filled KV cache for the trainer's model: batch x max_seq rows. */
 int ctd_kvcache_create(ctd_trainer_t t, int64_t batch, int64_t max_seq, ctd_kvcache_t* out);
+/* The same with rows held in `bits` bits: 32, or 4 (nn::KVCache::allocate). */
+int ctd_kvcache_create_bits(ctd_trainer_t t, int64_t batch, int64_t max_seq, int32_t bits,
+                            ctd_kvcache_t* out);
 int ctd_kvcache_destroy(ctd_kvcache_t c);
 int ctd_kvcache_len(ctd_kvcache_t c, int64_t* current_len);
 /* Model::forward(ids [B,T] host int64, cache (NULL: none), position_start)
@@ -226,6 +233,11 @@ int ctd_trainer_generate(ctd_trainer_t t, const int64_t* prompt, int64_t P, int3
                          float temperature, int32_t top_k, float top_p, uint64_t seed,
                          int64_t max_seq, int64_t* tokens, double* prefill_ms,
                          double* decode_ms);
+/* The same with a KV cache of kv_bits (32 or 4). */
+int ctd_trainer_generate_bits(ctd_trainer_t t, const int64_t* prompt, int64_t P, int32_t max_new,
+                              float temperature, int32_t top_k, float top_p, uint64_t seed,
+                              int64_t max_seq, int32_t kv_bits, int64_t* tokens,
+                              double* prefill_ms, double* decode_ms);
 
 /* Rows per chunk of the fused LM head + loss (ops::set_linear_cross_entropy_chunk_rows;
  * 0 = automatic). */

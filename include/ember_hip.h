@@ -415,6 +415,20 @@ int ember_attn_kv4(const float* q, const uint32_t* k_codes, const float* k_param
                    int64_t H, int64_t Hk, int64_t D, int64_t L, int64_t pos, int64_t S,
                    float scale, void* workspace, size_t workspace_bytes, ember_stream_t s);
 
+/* ember_attn_decode_qkv over a 4-bit cache: q [B,T,H,D] and k, v [B,T,Hk,D] are
+ * the raw projections of a decode step; the normalised (skipped when the weight
+ * is NULL), rotated k and v are quantised into cache rows [pos, pos + T), and o
+ * is ember_attn_kv4 of the normalised, rotated q over rows [0, pos + T).  T <=
+ * 8, H / Hk <= 32, D in {64, 128}; S <= 2^30, pos + T <= S (EMBER_EINVAL);
+ * alignment as above, norm weights 16 bytes; `workspace` >=
+ * ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, pos + T). */
+int ember_attn_kv4_qkv(const float* q, const float* k, const float* v, int64_t B, int64_t T,
+                       int64_t H, int64_t Hk, int64_t D, const float* q_norm_w,
+                       const float* k_norm_w, float eps, const float* freqs_host, int64_t pos,
+                       uint32_t* k_codes, float* k_params, uint32_t* v_codes, float* v_params,
+                       int64_t S, float scale, float* o, void* workspace, size_t workspace_bytes,
+                       ember_stream_t s);
+
 /* ------------------------------------------------------ fused decode step
  * Kernels for calls of at most 8 token rows (decode), each streaming its
  * weights once with the small ops around it folded in.  No counterpart kernel

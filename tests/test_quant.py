@@ -1,11 +1,15 @@
 """CPU checks of the few-bit stores: the oracle's own rule, and the refusals of the entry points
 (no GPU compute is launched: every call here is rejected, or has nothing to do)."""
 import ctypes as C
+import json
+import os
+import subprocess
 
 import numpy as np
 import pytest
 
 from emberlm_amd import capi
+from emberlm_amd import trainer as TR
 from oracle import quant as OQ
 
 P = C.c_void_p(4096)      # never dereferenced
@@ -91,6 +95,45 @@ def test_attention_refusals():
     assert attn(L=4096, pos=4095, S=4096, ws=ODD, wsb=need) == -3
     assert capi.lib().ember_attn_kv4_workspace_bytes(1, 1, 4, 2, 64, 32) == 0
     assert capi.lib().ember_attn_kv4_workspace_bytes(1, 1, 4, 3, 64, 4096) == 0
+
+
+def test_decode_step_refusals():
+    f = (C.c_float * 64)()
+
+    def step(T=1, H=4, Hk=2, D=64, pos=0, S=8, B=1, freqs=f, **ptr):
+        a = {n: ptr.get(n, P) for n in ("q", "k", "v", "qn", "kn", "kc", "kp", "vc", "vp", "o")}
+        return capi.lib().ember_attn_kv4_qkv(
+            a["q"], a["k"], a["v"], B, T, H, Hk, D, a["qn"], a["kn"], 1e-6, freqs, pos, a["kc"],
+            a["kp"], a["vc"], a["vp"], S, 1.0, a["o"], None, 0, None)
+
+    assert step(T=2, pos=7) == -1 and step(T=9, S=16) == -1 and step(pos=-1) == -1
+    assert step(D=96) == -1 and step(H=3) == -1 and step(H=66) == -1 and step(freqs=None) == -1
+    assert step(S=2 ** 30 + 1) == -1 and step(B=-1) == -1 and step(pos=2 ** 63 - 1) == -1
+    for name in ("q", "k", "v", "kc", "kp", "vc", "vp", "o"):
+        assert step(**{name: None}) == -1, name
+        assert step(**{name: ODD}) == -3, name
+    assert step(qn=HALF) == -3 and step(kn=HALF) == -3
+    assert step(B=0) == 0 and step(T=0) == 0
+    assert step(pos=4000, S=4096) == -2  # split keys, no workspace
+
+
+@pytest.mark.parametrize("req,msg", [('"kv_bits": 8', "kv_bits must be 32 or 4"),
+                                     ('"kv_bits": "4"', "kv_bits must be an integer")])
+def test_generate_request_with_other_bits(req, msg):
+    exe = os.path.join(os.path.dirname(TR.LIB_PATH), "ctd_generate")
+    r = subprocess.run([exe, "--model", "/nonexistent.safetensors"],
+                       input='{"input_ids": [1], %s}' % req, capture_output=True, text=True,
+                       timeout=60)
+    assert r.returncode == 1 and msg in json.loads(r.stdout)["error"]
+
+
+@pytest.mark.parametrize("extra", ['"checkpoint_bits": 4, "gradient_checkpointing": true',
+                                   '"checkpoint_bits": 8'])
+def test_train_config_with_other_bits(tmp_path, extra):
+    cfg = tmp_path / "config.json"
+    cfg.write_text('{"init_weights": "w", "data_dir": "d", %s}' % extra)
+    with pytest.raises(TR.CtdError, match="checkpoint_bits"):
+        TR.train_run(cfg)
 
 
 def test_rows8_refusals_and_sizes():
