@@ -10,6 +10,7 @@
 //   q . k = step (q . c) + lo sum(q),
 // and a value row adds p lo + (p step) c to the output.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "quant.h"
@@ -24,7 +25,9 @@ constexpr int kMaxD = 256;  // of write and read; the attention takes 64 and 128
 
 // ------------------------------------------------------------ write, read
 // src rows [B,T,Hk,D] (blockIdx.y: keys or values) -> cache rows pos + t.
-// LPR lanes per row (a power of two >= D/8), eight values a lane.
+// LPR lanes per row (a power of two >= D/8), eight values a lane.  I: row
+// numbers, 32-bit wherever they fit (a 64-bit division costs as much as
+// quantising the lane's values).
 struct WriteArgs {
   const float* src[2];
   uint32_t* codes[2];
@@ -33,29 +36,27 @@ struct WriteArgs {
   int words;  // D / 8
 };
 
-template <int LPR>
+template <int LPR, typename I>
 __global__ __launch_bounds__(kThreads) void kv4_write_kernel(WriteArgs a) {
   const int z = blockIdx.y;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / LPR);
+  const I rows = static_cast<I>(a.rows), T = static_cast<I>(a.T), Hk = static_cast<I>(a.Hk);
+  const I step = static_cast<I>(gridDim.x) * (kThreads / LPR);
   const int w = threadIdx.x % LPR;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads / LPR); base < a.rows;
-       base += step) {
-    const int64_t r = base + threadIdx.x / LPR;
-    const bool live = r < a.rows && w < a.words;
+  for (I base = static_cast<I>(blockIdx.x) * (kThreads / LPR); base < rows; base += step) {
+    const I r = base + threadIdx.x / LPR;
+    const bool live = r < rows && w < a.words;
     float v[8] = {};
+    float lo = INFINITY, hi = -INFINITY;
+    bool bad = false;
     if (live) {
-      const f32x4* p =
-          reinterpret_cast<const f32x4*>(a.src[z] + (r * a.words + w) * 8);
+      const f32x4* p = reinterpret_cast<const f32x4*>(
+          a.src[z] + (static_cast<int64_t>(r) * a.words + w) * 8);
       const f32x4 x = p[0], y = p[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = x[e];
         v[4 + e] = y[e];
       }
-    }
-    float lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
-    if (live) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         lo = fminf(lo, v[e]);
@@ -64,40 +65,40 @@ __global__ __launch_bounds__(kThreads) void kv4_write_kernel(WriteArgs a) {
       }
     }
     const QuantGrid g = quant_grid<LPR, 15>(lo, hi, bad);
+    unsigned c[8];
+    quant_codes<15>(g, v, c);
     if (!live) continue;
     uint32_t word = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) word |= quant_code<15>(g, v[e]) << (4 * e);
-    const int64_t h = r % a.Hk, t = r / a.Hk % a.T, b = r / (a.Hk * a.T);
-    const int64_t row = (b * a.Hk + h) * a.S + a.pos + t;
+    for (int e = 0; e < 8; ++e) word |= c[e] << (4 * e);
+    const I bt = r / Hk, b = bt / T;
+    const int64_t row = (static_cast<int64_t>(b) * Hk + (r - bt * Hk)) * a.S + a.pos + (bt - b * T);
     a.codes[z][row * a.words + w] = word;
     if (w == 0) *reinterpret_cast<float2*>(a.params[z] + 2 * row) = float2{g.lo, g.step};
   }
 }
 
-__device__ __forceinline__ void held8(uint32_t word, float2 p, float (&x)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    x[e] = fmaf(static_cast<float>((word >> (4 * e)) & 15u), p.y, p.x);
-}
-
-// Cache rows [0, L) -> out [B, Hk*group, L, D]; a thread reads one word and
-// writes its eight values to every head of the group.
+// Cache rows [0, L) -> out [B, Hk*group, L, D]; a thread reads half a word and
+// writes its four values to every head of the group, 16 bytes beside its
+// neighbour's.
+template <typename I>
 __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
     const uint32_t* __restrict__ codes, const float* __restrict__ params, float* __restrict__ out,
     int64_t n, int64_t group, int64_t L, int64_t S, int words) {
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+  const I stride = static_cast<I>(gridDim.x) * kThreads;
+  const I per = static_cast<I>(2 * words), rows = static_cast<I>(L);
+  for (I i = static_cast<I>(blockIdx.x) * kThreads + threadIdx.x; i < static_cast<I>(n);
        i += stride) {
-    const int64_t w = i % words, j = i / words % L, bh = i / (words * L);
-    const int64_t row = bh * S + j;
-    float x[8];
-    held8(codes[row * words + w], *reinterpret_cast<const float2*>(params + 2 * row), x);
-    for (int64_t h = 0; h < group; ++h) {
-      f32x4* o = reinterpret_cast<f32x4*>(out) + (((bh * group + h) * L + j) * words + w) * 2;
-      o[0] = f32x4{x[0], x[1], x[2], x[3]};
-      o[1] = f32x4{x[4], x[5], x[6], x[7]};
-    }
+    const I rj = i / per, c = i - rj * per, bh = rj / rows, j = rj - bh * rows;
+    const int64_t row = static_cast<int64_t>(bh) * S + j;
+    const uint32_t w = codes[row * words + (c >> 1)] >> (16 * (c & 1));
+    const float2 p = *reinterpret_cast<const float2*>(params + 2 * row);
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fmaf(static_cast<float>((w >> (4 * e)) & 15u), p.y, p.x);
+    f32x4* o = reinterpret_cast<f32x4*>(out) +
+               (static_cast<int64_t>(bh) * group * L + j) * per + c;
+    for (int64_t h = 0; h < group; ++h) o[h * L * per] = x;
   }
 }
 
@@ -367,6 +368,8 @@ struct Fold {
   float freqs[kMaxRopePairs];
 };
 
+struct NoFold {};
+
 // A query row's D/4 values per lane (dims g D/4 ..): RMSNorm, then the
 // rotation of the pairs (c, c + D/2), whose second halves lie two lane groups on.
 template <int D>
@@ -443,10 +446,12 @@ __device__ __forceinline__ void fold_rows(const AttnArgs& a, const Fold& f,
     bad |= not_finite(x[e]);
   }
   const QuantGrid g = quant_grid<LPR, 15>(lo, hi, bad);
+  unsigned c[8];
+  quant_codes<15>(g, x, c);
   if (!live || !mine(a.pos + t)) return;
   uint32_t word = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) word |= quant_code<15>(g, x[e]) << (4 * e);
+  for (int e = 0; e < 8; ++e) word |= c[e] << (4 * e);
   const int64_t row = bh * a.S + a.pos + t;
   (value ? f.vc : f.kc)[row * LPR + w] = word;
   if (w == 0)
@@ -466,7 +471,8 @@ __device__ __forceinline__ void fold_rows(const AttnArgs& a, const Fold& f,
 // of that head reads them, except those of another row tile, which write the
 // same bits themselves.
 template <int D, int NT, int WAVES, bool FOLD>
-__global__ __launch_bounds__(kWave * WAVES, 8 / WAVES) void attn_kv4_narrow(AttnArgs a, Fold f) {
+__global__ __launch_bounds__(kWave * WAVES, 8 / WAVES) void attn_kv4_narrow(
+    AttnArgs a, std::conditional_t<FOLD, Fold, NoFold> f) {
   constexpr int W = D / 8, S = D / 32, ND = D / 16, ROWS = 16 * NT;
   constexpr int kThreads = kWave * WAVES, kWaves = WAVES;
   constexpr int VS = W + 4;                       // words per V row in LDS
@@ -935,6 +941,10 @@ Plan attn_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t L) {
   return Plan{variant, static_cast<int>(want), row_tiles};
 }
 
+// Below this a 32-bit index does not wrap when a grid's stride (at most 2^28) is
+// added to it.
+constexpr int64_t kIndex32 = int64_t{1} << 31;
+
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 }  // namespace
@@ -954,7 +964,10 @@ extern "C" int ember_kv4_write(const float* k, const float* v, uint32_t* k_codes
   auto launch = [&](auto lpr) {
     constexpr int LPR = decltype(lpr)::value;
     const dim3 grid(grid_1d(a.rows, kThreads / LPR), 2);
-    kv4_write_kernel<LPR><<<grid, kThreads, 0, as_stream(s)>>>(a);
+    if (a.rows < kIndex32)
+      kv4_write_kernel<LPR, uint32_t><<<grid, kThreads, 0, as_stream(s)>>>(a);
+    else
+      kv4_write_kernel<LPR, int64_t><<<grid, kThreads, 0, as_stream(s)>>>(a);
   };
   if (a.words <= 8)
     launch(std::integral_constant<int, 8>{});
@@ -970,12 +983,18 @@ extern "C" int ember_kv4_read_expanded(const uint32_t* codes, const float* param
                                        int64_t S, ember_stream_t s) {
   if (B < 0 || Hk < 0 || group <= 0 || L < 0 || L > S) return EMBER_EINVAL;
   if (D < 8 || D > kMaxD || D % 8) return EMBER_EINVAL;
-  const int64_t n = B * Hk * L * (D / 8);
+  const int64_t n = B * Hk * L * (D / 4);
   if (n == 0) return EMBER_OK;
   if (!codes || !params || !out) return EMBER_EINVAL;
   if (!aligned16(codes) || !aligned16(out) || !aligned8(params)) return EMBER_EALIGN;
-  kv4_read_expanded_kernel<<<grid_1d(n, kThreads), kThreads, 0, as_stream(s)>>>(
-      codes, params, out, n, group, L, S, static_cast<int>(D / 8));
+  const unsigned grid = grid_1d(n, kThreads);
+  const int words = static_cast<int>(D / 8);
+  if (n < kIndex32)
+    kv4_read_expanded_kernel<uint32_t>
+        <<<grid, kThreads, 0, as_stream(s)>>>(codes, params, out, n, group, L, S, words);
+  else
+    kv4_read_expanded_kernel<int64_t>
+        <<<grid, kThreads, 0, as_stream(s)>>>(codes, params, out, n, group, L, S, words);
   return launch_status();
 }
 
@@ -1024,7 +1043,8 @@ int run_attn(const float* q, const uint32_t* kc, const float* kp, const uint32_t
   auto launch = [&](auto d, auto folded) {
     constexpr int DD = decltype(d)::value;
     constexpr bool FOLD = decltype(folded)::value;
-    const Fold f = fold ? *fold : Fold{};
+    std::conditional_t<FOLD, Fold, NoFold> f;
+    if constexpr (FOLD) f = *fold;
     const dim3 grid(static_cast<unsigned>(blocks));
     if (p.variant == kOne)
       attn_kv4_narrow<DD, 1, kOneWaves, FOLD><<<grid, kWave * kOneWaves, 0, st>>>(a, f);

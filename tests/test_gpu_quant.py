@@ -297,8 +297,8 @@ def test_attention_captured_and_on_another_stream(T, L):
 
 
 # --------------------------------------------------------------------------- 8-bit rows
-ROWS = [(1, 1), (3, 7), (5, 64), (2, 127), (4, 128), (7, 129), (3, 200), (11, 576), (6, 960),
-        (5, 1001), (4, 2048), (2, 5000), (600, 36), (2, 8200)]
+ROWS = [(2100, 36), (2050, 300), (2049, 1030), (2048, 2500), (1, 1), (3, 7), (5, 64), (2, 127), (4, 128), (7, 129), (3, 200), (11, 576), (6, 960),
+        (5, 1001), (4, 2048), (2, 5000), (600, 36), (2, 8200), (2048, 17), (2060, 100)]
 
 
 def quantised(x, offset=0):
