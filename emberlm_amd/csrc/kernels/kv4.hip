@@ -116,11 +116,13 @@ __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
 // where q' = q 2^(15 - ex) is a query scaled by a power of two so that its
 // largest element lies in [2^14, 2^15): its low pieces then stay normal f16.
 // The softmax runs against a reference per query
-//   ref = max_j (score_j + e_j - 14),  2^e_j > step of value row j,
+//   ref ~ max_j (score_j + e_j - 8),  2^e_j > step of value row j,
 // instead of max score_j, so that the weights p_j = 2^(score_j - ref) times
-// their steps stay below 2^14 and near it: the f16 range again, whatever the
-// rows' sizes.  e_j is at least -60, which bounds p_j by 2^74 where steps
-// vanish.  A query's bits depend on the rows it sees only.
+// their steps have their largest between 2^7 and 2^15 (ref may trail the
+// maximum by kMargin): the f16 range again, whatever the rows' sizes.  A weight
+// 2^-11 of the largest or more keeps its 22 bits, a smaller one is off by less
+// than 2^-33 of the largest.  e_j is at least -60, which bounds p_j by 2^75 where
+// steps vanish.  A query's bits depend on the rows it sees only.
 //
 // Fragments (lane = (g = lane / 16, i = lane % 16)):
 //   S^T = K Q^T: A holds key i, dims g D/4 + 8 s + {0,4,1,5,2,6,3,7} in step s (the
@@ -138,6 +140,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlockKeys = 32;  // keys of one softmax step
+constexpr int kMinExp = -60, kShift = 8;
+constexpr float kMargin = 7.f;
 constexpr int kMaxSplits = 512;
 constexpr int64_t kMaxRows = 1 << 30;  // of a cache: row numbers are 32-bit in the kernels
 
@@ -263,19 +267,25 @@ __device__ __forceinline__ void stage_params(float* par, int key, bool value, fl
   par[(value ? kVStep : kKStep) * KEYS + key] = step;
   par[(value ? kVLo : kKLo) * KEYS + key] = lo8;
   if (value) {
-    const int ex = step > 0.f && !not_finite(step) ? __builtin_amdgcn_frexp_expf(step) : -60;
-    par[kVExp * KEYS + key] = static_cast<float>((ex > -60 ? ex : -60) - 14);
+    const int ex = step > 0.f && !not_finite(step) ? __builtin_amdgcn_frexp_expf(step) : kMinExp;
+    par[kVExp * KEYS + key] = static_cast<float>((ex > kMinExp ? ex : kMinExp) - kShift);
   }
 }
 
-// One block of 32 keys for one query tile: the products s[kt] become weights,
-// in place; returns what the accumulators are to be multiplied by.  par: the
-// block's first key in the arrays of KEYS floats.  vis: how many keys from
-// this lane's first (4 g) on the query sees; MASK: some query does not see all.
-template <int KEYS, bool MASK>
-__device__ __forceinline__ float soften(f32x4 (&s)[2], const float* par, int g, int vis, float qmul,
-                                        float qsum, Softmax& st) {
-  float z = -INFINITY;
+// One block of 32 keys for NT query tiles, in two steps; the tiles go through
+// them together, so that their parameters are read once and their chains of
+// arithmetic overlap.  par: the block's first key in the arrays of KEYS floats.
+// vis: how many keys from this lane's first (4 g) on each tile's query sees;
+// MASK: some query does not see all.
+//
+// score: the products s[n][kt] become scores, in place, hidden ones -inf; z[n]
+// the largest of a query's scores plus exponents.
+template <int KEYS, bool MASK, int D, int NT>
+__device__ __forceinline__ void score(f32x4 (&s)[NT][2], const float* par, int g,
+                                      const int (&vis)[NT], const QRow<D> (&q)[NT],
+                                      float (&z)[NT]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) z[n] = -INFINITY;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
     const float* p = par + 16 * kt + 4 * g;
@@ -283,41 +293,81 @@ __device__ __forceinline__ float soften(f32x4 (&s)[2], const float* par, int g, 
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p + kKLo * KEYS);
     const f32x4 ex = *reinterpret_cast<const f32x4*>(p + kVExp * KEYS);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[kt][e] = fmaf(s[kt][e] * qmul, step[e], qsum * lo[e]);
-      if (MASK && 16 * kt + e >= vis) s[kt][e] = -INFINITY;
-      z = fmaxf(z, s[kt][e] + ex[e]);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][kt][e] = fmaf(s[n][kt][e] * q[n].mul, step[e], q[n].sum * lo[e]);
+        if (MASK && 16 * kt + e >= vis[n]) s[n][kt][e] = -INFINITY;
+        z[n] = fmaxf(z[n], s[n][kt][e] + ex[e]);
+      }
   }
-  const float ref = fmaxf(st.ref, max_over_rows(z));
+#pragma unroll
+  for (int n = 0; n < NT; ++n) z[n] = max_over_rows(z[n]);
+}
+
+// soften: scores become weights times steps, in two f16 pieces.
+template <int KEYS, bool MASK, int NT>
+__device__ __forceinline__ void soften(f32x4 (&s)[NT][2], const float* par, int g,
+                                       const int (&vis)[NT], Softmax (&st)[NT],
+                                       half8_t (&hi)[NT], half8_t (&lo8)[NT]) {
+  float r[NT], x[NT][8];
   // no key seen yet: any finite reference gives weights of 0
-  const float r = ref == -INFINITY ? 0.f : ref;
-  const float alpha = __builtin_amdgcn_exp2f(st.ref - r);
-  float l = 0.f, olo = 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) r[n] = st[n].ref == -INFINITY ? 0.f : st[n].ref;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
     const float* p = par + 16 * kt + 4 * g;
     const f32x4 step = *reinterpret_cast<const f32x4*>(p + kVStep * KEYS);
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p + kVLo * KEYS);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool hidden = MASK && 16 * kt + e >= vis;
-      const float w = __builtin_amdgcn_exp2f(s[kt][e] - r);
-      l += w;
-      // a row that the query does not see may hold NaN
-      olo = hidden ? olo : fmaf(w, lo[e], olo);
-      s[kt][e] = hidden ? 0.f : w * step[e];
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool hidden = MASK && 16 * kt + e >= vis[n];
+        const float w = __builtin_amdgcn_exp2f(s[n][kt][e] - r[n]);
+        st[n].l += w;
+        // a row that the query does not see may hold NaN
+        st[n].olo = hidden ? st[n].olo : fmaf(w, lo[e], st[n].olo);
+        x[n][4 * kt + e] = hidden ? 0.f : w * step[e];
+      }
   }
-  st.l = st.l * alpha + l;
-  st.olo = st.olo * alpha + olo;
-  st.ref = ref;
-  return alpha;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) split_f16(x[n], hi[n], lo8[n]);
 }
 
-__device__ __forceinline__ void weights(const f32x4 (&s)[2], half8_t& hi, half8_t& lo) {
-  const float x[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
-  split_f16(x, hi, lo);
+// A block's weights in pieces.  The references move, and the accumulators are
+// rescaled, only where some query's largest score passes its reference by more
+// than kMargin (the weights times steps then still fit in f16); that stands
+// outside of the two forms, or the compiler keeps two sets of accumulators.
+template <int KEYS, int D, int NT, int ND>
+__device__ __forceinline__ void softmax_block(bool mask, f32x4 (&s)[NT][2], const float* par,
+                                              int g, const int (&vis)[NT], const QRow<D> (&q)[NT],
+                                              Softmax (&st)[NT], f32x4 (&acc)[NT][ND],
+                                              half8_t (&hi)[NT], half8_t (&lo)[NT]) {
+  float z[NT];
+  if (mask)
+    score<KEYS, true>(s, par, g, vis, q, z);
+  else
+    score<KEYS, false>(s, par, g, vis, q, z);
+  bool past = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) past |= z[n] > st[n].ref + kMargin;
+  if (__any(past)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float ref = fmaxf(st[n].ref, z[n]);
+      const float alpha = ref == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[n].ref - ref);
+      st[n].l *= alpha;
+      st[n].olo *= alpha;
+      st[n].ref = ref;
+#pragma unroll
+      for (int t = 0; t < ND; ++t) acc[n][t] *= alpha;
+    }
+  }
+  if (mask)
+    soften<KEYS, true>(s, par, g, vis, st, hi, lo);
+  else
+    soften<KEYS, false>(s, par, g, vis, st, hi, lo);
 }
 
 // The weight of a partial result with reference m and weight sum l against M.
@@ -354,6 +404,7 @@ __device__ __forceinline__ int64_t clamp_row(int j, int L) { return min(j, L - 1
 
 // A decode step's norms, rotations and cache write (ember_attn_kv4_qkv).
 constexpr int kFoldRows = 8;       // new rows per call (T)
+constexpr int kFoldGroup = 32;     // query heads per KV head
 constexpr int kMaxRopePairs = 64;  // D <= 128
 struct Fold {
   const float* kn;    // [B, T, Hk, D] key projection
@@ -471,7 +522,7 @@ __device__ __forceinline__ void fold_rows(const AttnArgs& a, const Fold& f,
 // of that head reads them, except those of another row tile, which write the
 // same bits themselves.
 template <int D, int NT, int WAVES, bool FOLD>
-__global__ __launch_bounds__(kWave * WAVES, 8 / WAVES) void attn_kv4_narrow(
+__global__ __launch_bounds__(kWave * WAVES, 2) void attn_kv4_narrow(
     AttnArgs a, std::conditional_t<FOLD, Fold, NoFold> f) {
   constexpr int W = D / 8, S = D / 32, ND = D / 16, ROWS = 16 * NT;
   constexpr int kThreads = kWave * WAVES, kWaves = WAVES;
@@ -585,28 +636,26 @@ __global__ __launch_bounds__(kWave * WAVES, 8 / WAVES) void attn_kv4_narrow(
     __builtin_amdgcn_wave_barrier();
     if (j0 + j_step < jend) load(j0 + j_step);
 
-    half8_t ph[NT], pl[NT];
+    f32x4 s[NT][2];
+    int vis[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int k = 0; k < S; ++k) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma(kf[kt][k], q[n].hi[k], s[kt]);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma(kf[kt][k], q[n].lo[k], s[kt]);
-      }
-      const int vis = lim[n] - j0 - 4 * g;
-      const float alpha =
-          j0 + kBlockKeys > jall
-              ? soften<kBlockKeys, true>(s, par, g, vis, q[n].mul, q[n].sum, st[n])
-              : soften<kBlockKeys, false>(s, par, g, vis, q[n].mul, q[n].sum, st[n]);
-      weights(s, ph[n], pl[n]);
-      if (__any(alpha != 1.f)) {
-#pragma unroll
-        for (int t = 0; t < ND; ++t) acc[n][t] *= alpha;
-      }
+      s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      vis[n] = lim[n] - j0 - 4 * g;
     }
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[n][kt] = mfma(kf[kt][k], q[n].hi[k], s[n][kt]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[n][kt] = mfma(kf[kt][k], q[n].lo[k], s[n][kt]);
+    }
+    half8_t ph[NT], pl[NT];
+    softmax_block<kBlockKeys>(j0 + kBlockKeys > jall, s, par, g, vis, q, st, acc, ph, pl);
     // V words of this lane's eight keys, then a half (D = 128: both) of each.
     uint32_t vx[8];
 #pragma unroll
@@ -687,9 +736,9 @@ __global__ __launch_bounds__(kWave * WAVES, 8 / WAVES) void attn_kv4_narrow(
 }
 
 // Many query rows: a workgroup owns 128 rows, 32 to a wave, and one key split.
-// Tiles of 64 keys are unpacked once, each wave a quarter, into two LDS
-// buffers that hold them as fragments, 16 bytes per lane one after another, so
-// that every wave's reads are free of bank conflicts; the next tile's codes are
+// Tiles of 64 keys are unpacked once, each wave a quarter, into two LDS buffers
+// that hold them as fragments, 16 bytes per lane one after another, so that
+// every wave's reads are free of bank conflicts; the next tile's codes are
 // loaded during a tile and unpacked after it.
 constexpr int kWideRows = 128;
 constexpr int kTileKeys = 64;
@@ -720,13 +769,11 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
   const uint32_t* kc = a.kc + it.bh * a.S * W;
   const uint32_t* vc = a.vc + it.bh * a.S * W;
   const float2* pp = reinterpret_cast<const float2*>(w == 0 ? a.kp : a.vp) + it.bh * a.S;
-
   u32x4 kw;
   uint32_t vw[4];
   float2 pw = {0.f, 0.f};
   auto load = [&](int j0) {  // rows past the last key read that one again
-    const int64_t row = clamp_row(j0 + 16 * w + i, a.L);
-    const uint32_t* p = kc + row * W + g * S;
+    const uint32_t* p = kc + clamp_row(j0 + 16 * w + i, a.L) * W + g * S;
     if constexpr (S == 4) {
       kw = *reinterpret_cast<const u32x4*>(p);
     } else {
@@ -734,10 +781,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
       kw = u32x4{x[0], x[1], 0u, 0u};
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t vrow = clamp_row(j0 + 16 * w + 4 * g + e, a.L);
-      vw[e] = vc[vrow * W + (D == 128 ? i : i >> 1)];
-    }
+    for (int e = 0; e < 4; ++e)
+      vw[e] = vc[clamp_row(j0 + 16 * w + 4 * g + e, a.L) * W + (D == 128 ? i : i >> 1)];
     if (w < 2) pw = pp[clamp_row(j0 + lane, a.L)];
   };
   auto stage = [&](int buf, int j0) {
@@ -780,49 +825,37 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
   for (int j0 = ks; j0 < jend; j0 += j_step, buf ^= 1) {
     const bool more = j0 + j_step < jend;
     if (more) load(j0 + j_step);
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < kTileKeys / 32; ++u) {
       const int jb = j0 + 32 * u;
-      if (jb >= wend) continue;
+      if (jb >= wend) break;
       f32x4 s[NT][2];
+      int vis[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) s[n][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        vis[n] = lim[n] - jb - 4 * g;
+      }
 #pragma unroll
       for (int k = 0; k < S; ++k)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           const half8_t kf = kfrag[buf][2 * u + kt][k][lane];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            s[n][kt] = mfma(kf, q[n].hi[k], s[n][kt]);
-            s[n][kt] = mfma(kf, q[n].lo[k], s[n][kt]);
-          }
+          for (int n = 0; n < NT; ++n) s[n][kt] = mfma(kf, q[n].hi[k], s[n][kt]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[n][kt] = mfma(kf, q[n].lo[k], s[n][kt]);
         }
       half8_t ph[NT], pl[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float* pb = par[buf] + 32 * u;
-        const int vis = lim[n] - jb - 4 * g;
-        const float alpha =
-            jb + 32 > wall
-                ? soften<kTileKeys, true>(s[n], pb, g, vis, q[n].mul, q[n].sum, st[n])
-                : soften<kTileKeys, false>(s[n], pb, g, vis, q[n].mul, q[n].sum, st[n]);
-        weights(s[n], ph[n], pl[n]);
-        if (__any(alpha != 1.f)) {
-#pragma unroll
-          for (int t = 0; t < ND; ++t) acc[n][t] *= alpha;
-        }
-      }
+      const float* pb = par[buf] + 32 * u;
+      softmax_block<kTileKeys>(jb + 32 > wall, s, pb, g, vis, q, st, acc, ph, pl);
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
         const half8_t vf = vfrag[buf][u][t][lane];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][t] = mfma(vf, ph[n], acc[n][t]);
-          acc[n][t] = mfma(vf, pl[n], acc[n][t]);
-        }
+        for (int n = 0; n < NT; ++n) acc[n][t] = mfma(vf, ph[n], acc[n][t]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][t] = mfma(vf, pl[n], acc[n][t]);
       }
     }
     if (more) stage(buf ^ 1, j0 + j_step);
@@ -872,6 +905,15 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
   const float* ml = part_ml + static_cast<int64_t>(live ? row : 0) * nsplit * 2;
   const float* po = part_o + static_cast<int64_t>(live ? row : 0) * nsplit * D + 4 * c4;
   const int own = threadIdx.x % PER_ROW;
+  // The first kAhead of a group's partial rows are on their way while the
+  // weights are formed.
+  constexpr int kAhead = 4;
+  f32x4 x[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int s = min(part + u * PARTS, nsplit - 1);
+    x[u] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(s) * D);
+  }
   float M = -INFINITY;
   for (int s = own; s < nsplit; s += PER_ROW) M = fmaxf(M, ml[2 * s]);
   M = wave_max(M);
@@ -883,12 +925,17 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
   }
   float l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = part; s < nsplit; s += PARTS) {
+  auto add = [&](int s, f32x4 v) {
     const float ls = ml[2 * s + 1], e = merge_weight(ml[2 * s], ls, M);
     l += ls * e;
-    acc += *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(s) * D) * e;
-  }
+    acc += v * e;
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (part + u * PARTS < nsplit) add(part + u * PARTS, x[u]);
+#pragma unroll 4
+  for (int s = part + kAhead * PARTS; s < nsplit; s += PARTS)
+    add(s, *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(s) * D));
   s_o[threadIdx.x] = acc;
   s_l[threadIdx.x] = l;
   __syncthreads();
@@ -908,13 +955,17 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
 //    CU has a head of its own, one workgroup of eight waves per head and no second
 //    launch (257 keys 5.2 against 6.4 in splits of four waves, 512 keys 7.6 and
 //    7.3, 1024 keys 8.6 and 7.3; 256 heads of 4000 keys 33.9 and 36.0); else splits.
-//  - R <= kNarrowRows: two query tiles; beyond, the shared tiles of 128 rows.
+//  - beyond, two query tiles, each workgroup for itself; or the shared tiles of
+//    128 rows where there is so much to do that unpacking counts for more than
+//    their barriers, kWideWork rows times keys or more (512 rows: 16384 keys 92
+//    against 94, 32768 keys 165 and 156; 2048 rows: 4096 keys 78 and 84, 16384
+//    keys 303 and 281).
 //  - Splits: a workgroup for each CU, two where that leaves kLongKeys keys or more
 //    to each (130001 keys 36 against 42 with one; 4096 keys and 128 rows, where
 //    the partial results weigh more, 23 against 19), and 32 keys a wave at least.
 constexpr int64_t kCus = 256;
 constexpr int64_t kOneKeys = 512;
-constexpr int64_t kNarrowRows = 256;
+constexpr int64_t kWideWork = int64_t{1} << 24;
 constexpr int64_t kLongKeys = 1024;
 constexpr int kOneWaves = 8;
 
@@ -929,7 +980,8 @@ struct Plan {
 Plan attn_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t L) {
   const int64_t R = H / Hk * T, heads = B * Hk;
   if (R <= 16 && (L <= kOneKeys || heads >= kCus)) return Plan{kOne, 1, 1};
-  const Variant variant = R <= 16 ? kTile : R <= kNarrowRows ? kTwoTiles : kWide;
+  const bool wide = R > kFoldRows * kFoldGroup && R * L >= kWideWork;  // a decode step's never
+  const Variant variant = R <= 16 ? kTile : wide ? kWide : kTwoTiles;
   const int64_t rows = variant == kTile ? 16 : variant == kTwoTiles ? 32 : kWideRows;
   const int64_t unit = variant == kWide ? kWideKeys : kBlockKeys * kWaves;
   const int64_t row_tiles = (R + rows - 1) / rows, items = heads * row_tiles;
@@ -1052,10 +1104,8 @@ int run_attn(const float* q, const uint32_t* kc, const float* kp, const uint32_t
       attn_kv4_narrow<DD, 1, kWaves, FOLD><<<grid, kThreads, 0, st>>>(a, f);
     else if (p.variant == kTwoTiles)
       attn_kv4_narrow<DD, 2, kWaves, FOLD><<<grid, kThreads, 0, st>>>(a, f);
-    else if (!FOLD)
-      attn_kv4_wide<DD><<<grid, kThreads, 0, st>>>(a);
     else
-      return static_cast<int>(EMBER_EINVAL);
+      attn_kv4_wide<DD><<<grid, kThreads, 0, st>>>(a);
     const int rc = launch_status();
     if (rc || p.nsplit == 1) return rc;
     constexpr int kWaveParts = 256 / DD, kBlockParts = 1024 / DD;
@@ -1102,7 +1152,7 @@ extern "C" int ember_attn_kv4_qkv(const float* q, const float* k, const float* v
                                   ember_stream_t s) {
   if (B < 0 || T < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || pos < 0 || !freqs_host)
     return EMBER_EINVAL;
-  if ((D != 64 && D != 128) || T > kFoldRows || H / Hk > kNarrowRows / kFoldRows)
+  if ((D != 64 && D != 128) || T > kFoldRows || H / Hk > kFoldGroup)
     return EMBER_EINVAL;
   if (S > kMaxRows || T > S || pos > S - T) return EMBER_EINVAL;
   if (B == 0 || T == 0) return EMBER_OK;

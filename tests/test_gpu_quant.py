@@ -175,6 +175,7 @@ ATTEND = [  # B, T, H, Hk, D, L, pos, S
     (1, 33, 8, 8, 64, 1025, 992, 1030),
     (1, 5, 4, 2, 64, 20, 40, 64),           # every row past L's last key
     (1, 40, 4, 2, 128, 30, 3, 64),          # keys end before the queries do
+    (1, 300, 2, 2, 64, 700, 400, 701),      # ten tiles of 32 rows
 ]
 
 
@@ -197,6 +198,44 @@ def test_attention_over_kv4(B, T, H, Hk, D, L, pos, S):
         part = attend(q, cache, L, pos, D ** -0.5)
         assert same(part[:, :T // 2], got[:, :T // 2])
         assert np.isnan(part[:, T // 2:]).all()
+
+
+def attention64(q, k, v, pos, scale, L):
+    """OQ.attention on the GPU, in 64 bits, for sizes that take a while in numpy."""
+    q, k, v = (torch.from_numpy(np.ascontiguousarray(x)).cuda().double() for x in (q, k, v))
+    B, T, H, D = q.shape
+    g = H // k.shape[1]
+    seen = torch.arange(L, device="cuda")[None] > (pos + torch.arange(T, device="cuda"))[:, None]
+    o = torch.empty_like(q)
+    for b in range(B):
+        for h in range(H):
+            z = q[b, :, h] @ k[b, h // g, :L].T.contiguous() * scale
+            z[seen] = float("-inf")
+            o[b, :, h] = torch.softmax(z, 1) @ v[b, h // g, :L]
+    return o.cpu().numpy()
+
+
+@pytest.mark.parametrize("B,T,H,Hk,D,L,pos,S", [
+    (1, 600, 2, 2, 64, 28000, 27400, 28003),   # the shared tiles: 600 rows, ragged
+    (1, 2050, 4, 2, 128, 4200, 2150, 4200),    # 4100 rows
+    (2, 259, 2, 1, 128, 32500, 32241, 32500),  # the last tile holds 6 rows
+    (1, 4099, 1, 1, 64, 4099, 0, 4099),        # a whole prompt
+])
+def test_attention_of_long_chunks(B, T, H, Hk, D, L, pos, S):
+    r = rng(T)
+    q = r.standard_normal((B, T, H, D)).astype(np.float32)
+    cache = held_cache(r, B, Hk, S, D)
+    got = attend(q, cache, L, pos, D ** -0.5)
+    ref = attention64(q, cache[0][2], cache[1][2], pos, D ** -0.5, L)
+    worst, l2 = attention_bounds(q, cache, D ** -0.5, L)
+    err = np.abs(got - ref)
+    assert err.max() <= worst and np.linalg.norm(err) <= l2 * np.linalg.norm(ref)
+    # rows that only later queries see, and rows past the last, do not reach a query
+    cut = pos + T // 2
+    for _, par, _ in cache:
+        par[:, :, cut:] = np.nan
+    part = attend(q, cache, L, pos, D ** -0.5)
+    assert same(part[:, :T // 2], got[:, :T // 2]) and np.isnan(part[:, T // 2:]).all()
 
 
 @pytest.mark.parametrize("T", [1, 6, 70])
@@ -296,6 +335,29 @@ def test_attention_captured_and_on_another_stream(T, L):
     assert same(host(o), attend(q * np.float32(0.5), cache, L, L - T, 0.1))
 
 
+def test_kv4_cache_past_int32_offsets():
+    """Rows whose words lie past 2^31: written, and seen by a query over the whole cache.  All other
+    rows hold zeros, so the output is (sum e^s_j v_j) / (S - 3 + sum e^s_j) over the three."""
+    r = rng(8)
+    D, H, S, T = 128, 2, 2 ** 27 + 40, 3
+    kc, vc = (torch.zeros(S * D // 8, device="cuda", dtype=torch.int32) for _ in range(2))
+    kp, vp = (torch.zeros(S * 2, device="cuda") for _ in range(2))
+    k, v = (r.standard_normal((1, T, 1, D)).astype(np.float32) for _ in range(2))
+    kd, vd = dev(k), dev(v)
+    call("ember_kv4_write", p(kd), p(vd), p(kc), p(kp), p(vc), p(vp), 1, T, 1, D, S, S - T, None)
+    q = np.stack([k[0, 0, 0] * f for f in (1.0, 1.6)])[None, None].astype(np.float32)
+    qd, o = dev(q), empty((1, 1, H, D))
+    need = capi.lib().ember_attn_kv4_workspace_bytes(1, 1, H, 1, D, S)
+    ws = empty((need // 4,))
+    call("ember_attn_kv4", p(qd), p(kc), p(kp), p(vc), p(vp), p(o), 1, 1, H, 1, D, S, S - 1, S,
+         0.15, p(ws), need, None)
+    held = [OQ.values(*OQ.quantise(x[0, :, 0], 15)) for x in (k, v)]
+    e = np.exp(q[0, 0].astype(np.float64) @ held[0].T * 0.15)
+    ref = e @ held[1] / (S - T + e.sum(1))[:, None]
+    # the rows before add 2^27 ones in splits of fp32 sums of at most 2^18 / 16 terms per lane
+    assert np.abs(host(o)[0, 0] - ref).max() <= 1e-3 * np.abs(ref).max()
+
+
 # --------------------------------------------------------------------------- 8-bit rows
 ROWS = [(2100, 36), (2050, 300), (2049, 1030), (2048, 2500), (1, 1), (3, 7), (5, 64), (2, 127), (4, 128), (7, 129), (3, 200), (11, 576), (6, 960),
         (5, 1001), (4, 2048), (2, 5000), (600, 36), (2, 8200), (2048, 17), (2060, 100)]
@@ -362,3 +424,26 @@ def test_q8_rows_and_their_norm(rows, H, offset):
         assert (host(b)[:offset] == 5).all() and (host(b)[offset + rows * H:] == 5).all()
     call("ember_q8_dequantize_rmsnorm", *args, None, rows, H, eps, None)
     assert same(host(y), first)
+
+
+def test_q8_rows_past_int32_offsets():
+    rows, H = 2 ** 20 + 3, 2048
+    x = torch.randn((rows, H), device="cuda")
+    lib = capi.lib()
+    codes = torch.empty(lib.ember_q8_code_bytes(rows, H), device="cuda", dtype=torch.uint8)
+    params = torch.empty(lib.ember_q8_param_bytes(rows, H) // 4, device="cuda")
+    call("ember_q8_quantize", p(x), p(codes), p(params), rows, H, None)
+    tail = host(x[-4:])
+    ref_c, ref_p = OQ.quantise_rows8(tail)
+    assert same(host(codes[-4 * H:]).reshape(4, H), ref_c)
+    assert same(host(params[-4 * 32:]).reshape(ref_p.shape), ref_p)
+    x.zero_()
+    call("ember_q8_dequantize", p(codes), p(params), p(x), rows, H, None)
+    close_roundings(host(x[-4:]), OQ.values_rows8(ref_c, ref_p, H))
+    y, w = torch.zeros_like(x), torch.ones(H, device="cuda")
+    x.zero_()
+    call("ember_q8_dequantize_rmsnorm", p(codes), p(params), p(w), p(x), p(y), None, rows, H, 0.0,
+         None)
+    v = OQ.values_rows8(ref_c, ref_p, H)
+    close_roundings(host(x[-4:]), v)
+    close_roundings(host(y[-4:]), v / np.sqrt((v * v).mean(1, keepdims=True)), H / 2 + 8)

@@ -51,6 +51,7 @@ def test_cpp_api_tests():
     (1, 8, 4, 2, 128, 1020, 1030, False, 0.0),   # new rows in two splits
     (1, 8, 8, 1, 64, 700, 710, True, 0.0),       # 64 rows a KV head: two row tiles write them
     (2, 4, 32, 1, 128, 130, 134, False, 0.0),    # group 32: four row tiles
+    (1, 8, 32, 1, 64, 65600, 65608, False, 0.0), # the largest group over a long cache
     (300, 1, 4, 1, 64, 40, 41, False, 0.0),      # as many heads as fill the GPU
 ])
 def test_decode_attention_kv4_fold(B, T, H, Hk, D, pos, S, qk, factor):
