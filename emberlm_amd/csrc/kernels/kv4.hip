@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
 // it, so a product is two MFMAs into one fp32 accumulator.  Three bf16 pieces would
 // hold all 24 bits for half as many MFMAs again; the sums of D or L fp32 terms
 // around them round by more than the two bits.  With lo' = lo + 8 step,
-//   score_j = qmul (q' . (c_j - 8)) step_j + qsum lo'_j          (log2 units)
+//   score_j = qmul (step_j (q' . (c_j - 8)) + lo'_j sum(q'))     (log2 units)
 // where q' = q 2^(15 - ex) is a query scaled by a power of two so that its
 // largest element lies in [2^14, 2^15): its low pieces then stay normal f16.
 // The softmax runs against a reference per query
@@ -198,12 +198,14 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
 // x as two f16 pieces (pairs convert in one instruction).
 typedef float float2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split_f16(const float (&x)[8], half8_t& hi, half8_t& lo) {
+  float minus = -1.f;  // a register: x - hi is then one mixed-precision fma
+  asm("" : "+s"(minus));
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const half2_t h = __builtin_convertvector((float2_t{x[e], x[e + 1]}), half2_t);
     const half2_t l = __builtin_convertvector(
-        (float2_t{fmaf(static_cast<float>(h[0]), -1.f, x[e]),
-                  fmaf(static_cast<float>(h[1]), -1.f, x[e + 1])}),
+        (float2_t{fmaf(static_cast<float>(h[0]), minus, x[e]),
+                  fmaf(static_cast<float>(h[1]), minus, x[e + 1])}),
         half2_t);
     hi[e] = h[0];
     hi[e + 1] = h[1];
@@ -230,23 +232,24 @@ struct QRow {
     }
   }
   __device__ __forceinline__ void set(const float (&x)[D / 4], float qscale) {
-    float amax = 0.f, s = 0.f;
+    float amax = 0.f;
 #pragma unroll
-    for (int c = 0; c < D / 4; ++c) {
-      amax = fmaxf(amax, fabsf(x[c]));
-      s += x[c];
-    }
+    for (int c = 0; c < D / 4; ++c) amax = fmaxf(amax, fabsf(x[c]));
     amax = max_over_rows(amax);
-    sum = sum_over_rows(s) * qscale;
     const int ex = amax > 0.f && !not_finite(amax) ? __builtin_amdgcn_frexp_expf(amax) : 15;
     mul = ldexpf(qscale, ex - 15);
+    float s = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[8 * k + (e >> 1) + 4 * (e & 1)], 15 - ex);
+      for (int e = 0; e < 8; ++e) {
+        y[e] = ldexpf(x[8 * k + (e >> 1) + 4 * (e & 1)], 15 - ex);
+        s += y[e];
+      }
       split_f16(y, hi[k], lo[k]);
     }
+    sum = sum_over_rows(s);
   }
 };
 
@@ -278,8 +281,8 @@ __device__ __forceinline__ void stage_params(float* par, int key, bool value, fl
 // vis: how many keys from this lane's first (4 g) on each tile's query sees;
 // MASK: some query does not see all.
 //
-// score: the products s[n][kt] become scores, in place, hidden ones -inf; z[n]
-// the largest of a query's scores plus exponents.
+// score: the products s[n][kt] become scores over q.mul, in place; z[n] the
+// largest of a query's scores plus exponents.
 template <int KEYS, bool MASK, int D, int NT>
 __device__ __forceinline__ void score(f32x4 (&s)[NT][2], const float* par, int g,
                                       const int (&vis)[NT], const QRow<D> (&q)[NT],
@@ -296,9 +299,9 @@ __device__ __forceinline__ void score(f32x4 (&s)[NT][2], const float* par, int g
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][kt][e] = fmaf(s[n][kt][e] * q[n].mul, step[e], q[n].sum * lo[e]);
-        if (MASK && 16 * kt + e >= vis[n]) s[n][kt][e] = -INFINITY;
-        z[n] = fmaxf(z[n], s[n][kt][e] + ex[e]);
+        s[n][kt][e] = fmaf(s[n][kt][e], step[e], q[n].sum * lo[e]);
+        const float t = fmaf(s[n][kt][e], q[n].mul, ex[e]);
+        z[n] = fmaxf(z[n], MASK && 16 * kt + e >= vis[n] ? -INFINITY : t);
       }
   }
 #pragma unroll
@@ -306,10 +309,10 @@ __device__ __forceinline__ void score(f32x4 (&s)[NT][2], const float* par, int g
 }
 
 // soften: scores become weights times steps, in two f16 pieces.
-template <int KEYS, bool MASK, int NT>
-__device__ __forceinline__ void soften(f32x4 (&s)[NT][2], const float* par, int g,
-                                       const int (&vis)[NT], Softmax (&st)[NT],
-                                       half8_t (&hi)[NT], half8_t (&lo8)[NT]) {
+template <int KEYS, bool MASK, int D, int NT>
+__device__ __forceinline__ void soften(const f32x4 (&s)[NT][2], const float* par, int g,
+                                       const int (&vis)[NT], const QRow<D> (&q)[NT],
+                                       Softmax (&st)[NT], half8_t (&hi)[NT], half8_t (&lo8)[NT]) {
   float r[NT], x[NT][8];
   // no key seen yet: any finite reference gives weights of 0
 #pragma unroll
@@ -324,7 +327,8 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NT][2], const float* par, int 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool hidden = MASK && 16 * kt + e >= vis[n];
-        const float w = __builtin_amdgcn_exp2f(s[n][kt][e] - r[n]);
+        const float t = __builtin_amdgcn_exp2f(fmaf(s[n][kt][e], q[n].mul, -r[n]));
+        const float w = hidden ? 0.f : t;
         st[n].l += w;
         // a row that the query does not see may hold NaN
         st[n].olo = hidden ? st[n].olo : fmaf(w, lo[e], st[n].olo);
@@ -339,11 +343,15 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NT][2], const float* par, int 
 // rescaled, only where some query's largest score passes its reference by more
 // than kMargin (the weights times steps then still fit in f16); that stands
 // outside of the two forms, or the compiler keeps two sets of accumulators.
+// The wave goes first at the vector ALU while it is here: of two waves on a SIMD
+// one is then sooner back to feed the matrix core (1024 queries over 16384
+// keys 278 -> 259 us; first while it multiplies, 278).
 template <int KEYS, int D, int NT, int ND>
 __device__ __forceinline__ void softmax_block(bool mask, f32x4 (&s)[NT][2], const float* par,
                                               int g, const int (&vis)[NT], const QRow<D> (&q)[NT],
                                               Softmax (&st)[NT], f32x4 (&acc)[NT][ND],
                                               half8_t (&hi)[NT], half8_t (&lo)[NT]) {
+  __builtin_amdgcn_s_setprio(1);
   float z[NT];
   if (mask)
     score<KEYS, true>(s, par, g, vis, q, z);
@@ -365,9 +373,10 @@ __device__ __forceinline__ void softmax_block(bool mask, f32x4 (&s)[NT][2], cons
     }
   }
   if (mask)
-    soften<KEYS, true>(s, par, g, vis, st, hi, lo);
+    soften<KEYS, true>(s, par, g, vis, q, st, hi, lo);
   else
-    soften<KEYS, false>(s, par, g, vis, st, hi, lo);
+    soften<KEYS, false>(s, par, g, vis, q, st, hi, lo);
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // The weight of a partial result with reference m and weight sum l against M.
