@@ -972,6 +972,8 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
 //  - Splits: a workgroup for each CU, two where that leaves kLongKeys keys or more
 //    to each (130001 keys 36 against 42 with one; 4096 keys and 128 rows, where
 //    the partial results weigh more, 23 against 19), and 32 keys a wave at least.
+//    A prompt whose row tiles fill the GPU once, the later ones with twice the
+//    mean's keys, is split in two all the same (4096 queries and keys 220 -> 176).
 constexpr int64_t kCus = 256;
 constexpr int64_t kOneKeys = 512;
 constexpr int64_t kWideWork = int64_t{1} << 24;
@@ -996,6 +998,7 @@ Plan attn_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t L) {
   const int64_t row_tiles = (R + rows - 1) / rows, items = heads * row_tiles;
   int64_t want = (kCus + items - 1) / items;
   if (L / want >= kLongKeys) want = (2 * kCus + items - 1) / items;
+  if (wide && want == 1 && items < 4 * kCus && 2 * T >= L) want = 2;
   const int64_t units = (L + unit - 1) / unit;
   if (want > units) want = units;
   if (want > kMaxSplits) want = kMaxSplits;
