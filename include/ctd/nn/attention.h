@@ -66,7 +66,8 @@ struct Attention {
   // kv, this call's K/V go to cache rows [position_start, position_start+T)
   // and the queries attend over rows [0, position_start+T).  With a 4-bit
   // cache they attend over what it holds, their own rows included, so that a
-  // result does not depend on how the tokens were split into calls.
+  // result does not depend, beyond rounding, on how the tokens were split into
+  // calls.
   Tensor forward(const Tensor& x, KVLayer* kv = nullptr, int position_start = 0) const {
     return o_proj.forward(forward_context(x, kv, position_start));
   }

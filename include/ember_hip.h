@@ -228,7 +228,8 @@ int ember_qknorm_rope_bwd(const float* dy, const float* x, const float* w, const
  * single values.
  * ember_q8_dequantize restores the rows; ember_q8_dequantize_rmsnorm also
  * gives y = x * rstd * w, the restored rows' RMSNorm (rstd[rows] may be NULL),
- * what a decoder block's re-run starts with. */
+ * what a decoder block's re-run starts with; x and y must not overlap.  The two
+ * restore fewer than 2^31 rows (EMBER_EINVAL). */
 size_t ember_q8_code_bytes(int64_t rows, int64_t H);
 size_t ember_q8_param_bytes(int64_t rows, int64_t H);
 int ember_q8_quantize(const float* x, void* codes, float* params, int64_t rows, int64_t H,
@@ -404,8 +405,8 @@ int ember_kv4_read_expanded(const uint32_t* codes, const float* params, float* o
  * from one token to a chunk of a prompt.  The codes enter the products as they
  * are held; sums and softmax statistics are fp32.  Rows past a query's last
  * visible one do not reach its output, whatever they hold.  D in {64, 128};
- * 1 <= L <= S <= 2^30, pos <= 2^30; magnitudes of keys and values below 2^100;
- * alignment as above.  `workspace` >=
+ * 1 <= L <= S <= 2^30, T and pos <= 2^30; magnitudes of keys and values below
+ * 2^100; alignment as above.  `workspace` >=
  * ember_attn_kv4_workspace_bytes (0: none needed; EMBER_EWORKSPACE when
  * smaller) holds the partial results of key splits, merged in a fixed order:
  * deterministic. */

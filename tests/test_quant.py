@@ -82,7 +82,8 @@ def test_attention_refusals():
     assert attn(D=96) == -1 and attn(H=3) == -1 and attn(Hk=0) == -1 and attn(pos=-1) == -1
     assert attn(L=0) == -1 and attn(L=9) == -1 and attn(S=2 ** 30 + 1, L=4) == -1
     assert attn(pos=2 ** 30 + 1) == -1 and attn(pos=2 ** 63 - 1) == -1
-    assert attn(B=-1) == -1 and attn(T=-1) == -1
+    assert attn(B=-1) == -1 and attn(T=-1) == -1 and attn(T=2 ** 30 + 1) == -1
+    assert attn(B=2 ** 20, T=2 ** 10, H=4) == -1  # 2^32 query rows
     for name in ("q", "kc", "kp", "vc", "vp", "o"):
         assert attn(**{name: None}) == -1, name
         assert attn(**{name: ODD}) == -3, name
@@ -152,4 +153,4 @@ def test_rows8_refusals_and_sizes():
     assert q(P, HALF, P, 1, 4) == -3 and q(P, P, ODD, 1, 4) == -3
     assert d(HALF, P, P, 1, 4) == -3 and n(c=HALF) == -3 and n(p=ODD) == -3
     assert q(None, None, None, 0, 4) == 0 and d(None, None, None, 4, 0) == 0 and n(rows=0) == 0
-    assert n(rows=2 ** 31) == -1
+    assert n(rows=2 ** 31) == -1 and d(P, P, P, 2 ** 31, 4) == -1
