@@ -317,3 +317,116 @@ def test_8_bit_checkpoints_hold_less():
     # when the last block runs the inputs of at least 11 of the 12 are held
     assert peaks[32] - peaks[8] >= 10 * (saved - held), peaks
     tr.close()
+
+
+def test_train_driver_with_8_bit_checkpoints(tmp_path):
+    """ctd_train with "checkpoint_bits": 8: the first step's loss is the fp32 checkpoints' (the
+    forward pass is the same), the later ones follow other gradients, and a resumed run ends with
+    the same bits as one that was not stopped."""
+    from tests.test_gpu_driver import make_run, read_st, tr_cfg
+    tr = TR.Trainer(tr_cfg(), seed=3, init_std=0.05)
+    init = tmp_path / "init.safetensors"
+    tr.save(init)
+    tr.close()
+    r = rng(5)
+    data = tmp_path / "data"
+    data.mkdir()
+    doc = r.integers(0, 1000, 49).astype(np.int32)  # every document, so that every batch is the same
+    np.tile(doc, 6).tofile(data / "train.bin")
+    np.ones(6 * 49, np.int8).tofile(data / "train_mask.bin")
+    np.tile(doc, 2).tofile(data / "val.bin")
+    np.ones(2 * 49, np.int8).tofile(data / "val_mask.bin")
+    losses = {}
+    for bits in (32, 8):
+        run = make_run(tmp_path, f"bits{bits}", init, data, 4, checkpoint_bits=bits)
+        TR.train_run(run / "config.json")
+        lines = [json.loads(x) for x in (run / "loss.jsonl").read_text().splitlines()]
+        losses[bits] = [x["loss"] for x in lines if "loss" in x]
+        assert len(losses[bits]) >= 4 and np.isfinite(losses[bits]).all()
+    assert losses[8][0] == losses[32][0] and losses[8] != losses[32]
+    half = make_run(tmp_path, "resumed", init, data, 4, checkpoint_bits=8,
+                    resume=tmp_path / "bits8" / "ckpt_step_2.safetensors")
+    TR.train_run(half / "config.json")
+    a, b = (read_st(tmp_path / n / "final.safetensors") for n in ("bits8", "resumed"))
+    assert a.keys() == b.keys() and all(np.array_equal(a[k], b[k]) for k in a)
+
+
+# ------------------------------------------------------------ captured, and at once
+def step_buffers(r, B, H, Hk, D, S):
+    cache = held_cache(r, B, Hk, S, D)
+    return [words(cache[0][0]), dev(cache[0][1]), words(cache[1][0]), dev(cache[1][1])]
+
+
+def test_captured_steps_replay_and_two_streams_at_once():
+    """A captured run of the operators as a step uses them (a chunk written and attended to, a
+    decode step on top, a checkpoint stored and restored), replayed between eager work, and the
+    same eager calls on two streams at once, each with buffers of its own."""
+    r = rng(12)
+    B, T, H, Hk, D, S, pos = 1, 40, 8, 4, 128, 900, 700
+    freqs = (C.c_float * (D // 2))()
+    capi.check(capi.lib().ember_rope_freqs_host(freqs, D, 1e4, 0.0, 1.0, 4.0, 64))
+    ins = [dev(r.standard_normal(s).astype(np.float32))
+           for s in ((B, T, H, D), (B, T, Hk, D), (B, T, Hk, D), (B, 1, H, D), (B, 1, Hk, D),
+                     (B, 1, Hk, D), (300, 640), (640,))]
+    start = step_buffers(r, B, H, Hk, D, S)
+
+    class Set:
+        def __init__(self):
+            self.cache = [t.clone() for t in start]
+            self.o, self.o1 = empty((B, T, H, D)), empty((B, 1, H, D))
+            n = [capi.lib().ember_attn_kv4_workspace_bytes(B, t, H, Hk, D, p)
+                 for t, p in ((T, pos + T), (1, pos + T + 1))]
+            assert n[0] and n[1]
+            self.ws = [torch.full((x // 4,), float("nan"), device="cuda") for x in n]
+            self.codes = torch.empty(capi.lib().ember_q8_code_bytes(300, 640), device="cuda",
+                                     dtype=torch.uint8)
+            self.params = empty((300, 5, 2))
+            self.x, self.y, self.rstd = empty((300, 640)), empty((300, 640)), empty((300,))
+
+        def run(self):
+            st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+            c = [p(t) for t in self.cache]
+            capi.call("ember_kv4_write", p(ins[1]), p(ins[2]), *c, B, T, Hk, D, S, pos, st)
+            capi.call("ember_attn_kv4", p(ins[0]), *c, p(self.o), B, T, H, Hk, D, pos + T, pos, S,
+                      0.09, p(self.ws[0]), self.ws[0].numel() * 4, st)
+            capi.call("ember_attn_kv4_qkv", p(ins[3]), p(ins[4]), p(ins[5]), B, 1, H, Hk, D, None,
+                      None, 1e-6, freqs, pos + T, *c, S, 0.09, p(self.o1), p(self.ws[1]),
+                      self.ws[1].numel() * 4, st)
+            capi.call("ember_q8_quantize", p(ins[6]), p(self.codes), p(self.params), 300, 640, st)
+            capi.call("ember_q8_dequantize_rmsnorm", p(self.codes), p(self.params), p(ins[7]),
+                      p(self.x), p(self.y), p(self.rstd), 300, 640, 1e-5, st)
+
+        def out(self):
+            return [host(t) for t in (*self.cache, self.o, self.o1, self.codes, self.x, self.y,
+                                      self.rstd)]
+
+    def wipe(s):
+        for t in (s.o, s.o1, s.x, s.y, s.rstd, *s.ws):
+            t.zero_()
+        for t, f in zip(s.cache, start):
+            t.copy_(f)
+
+    first = Set()
+    first.run()
+    want = first.out()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        first.run()
+    other = Set()
+    for _ in range(3):
+        wipe(first)
+        graph.replay()
+        assert all(same(a, b) for a, b in zip(first.out(), want))
+        wipe(other)
+        other.run()
+        assert all(same(a, b) for a, b in zip(other.out(), want))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    wipe(first), wipe(other)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, stream in zip((first, other), streams):
+            with torch.cuda.stream(stream):
+                s.run()
+    for s in (first, other):
+        assert all(same(a, b) for a, b in zip(s.out(), want))
