@@ -984,6 +984,8 @@ constexpr int64_t kOneKeys = 512;
 constexpr int64_t kWideWork = int64_t{1} << 24;
 constexpr int64_t kLongKeys = 1024;
 constexpr int kOneWaves = 8;
+// A launch holds fewer than 2^32 threads.
+constexpr int64_t kMaxBlocks = (int64_t{1} << 32) / (kWave * kOneWaves) - 1;
 
 enum Variant { kOne, kTile, kTwoTiles, kWide };
 
@@ -1085,7 +1087,7 @@ int run_attn(const float* q, const uint32_t* kc, const float* kp, const uint32_t
   const Plan p = attn_plan(B, T, H, Hk, L);
   const int64_t blocks = B * Hk * p.row_tiles * p.nsplit;
   const int64_t rows = B * T * H;
-  if (blocks > 0x7fffffff || rows > 0x7fffffff) return EMBER_EINVAL;
+  if (blocks > kMaxBlocks || rows > 0x7fffffff) return EMBER_EINVAL;
   const size_t need = ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, L);
   if (need && (!workspace || workspace_bytes < need)) return EMBER_EWORKSPACE;
   if (need && !aligned16(workspace)) return EMBER_EALIGN;

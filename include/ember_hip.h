@@ -405,8 +405,9 @@ int ember_kv4_read_expanded(const uint32_t* codes, const float* params, float* o
  * from one token to a chunk of a prompt.  The codes enter the products as they
  * are held; sums and softmax statistics are fp32.  Rows past a query's last
  * visible one do not reach its output, whatever they hold.  D in {64, 128};
- * 1 <= L <= S <= 2^30, T and pos <= 2^30; magnitudes of keys and values below
- * 2^100; alignment as above.  `workspace` >=
+ * 1 <= L <= S <= 2^30, T and pos <= 2^30, fewer than 2^31 query rows and 2^23
+ * workgroups (each takes 16 rows of a KV head at least, or all it has;
+ * EMBER_EINVAL); magnitudes of keys and values below 2^100; alignment as above.  `workspace` >=
  * ember_attn_kv4_workspace_bytes (0: none needed; EMBER_EWORKSPACE when
  * smaller) holds the partial results of key splits, merged in a fixed order:
  * deterministic. */

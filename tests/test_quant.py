@@ -98,6 +98,11 @@ def test_attention_refusals():
     assert capi.lib().ember_attn_kv4_workspace_bytes(1, 1, 4, 3, 64, 4096) == 0
 
 
+def test_attention_of_more_workgroups_than_a_launch_holds():
+    assert attn(B=2 ** 23, H=1, Hk=1, pos=0) == -1  # eight waves per head, 2^32 threads
+    assert attn(B=2 ** 23, H=32, Hk=1, pos=0) == -1  # two tiles of 16 rows per workgroup
+
+
 def test_decode_step_refusals():
     f = (C.c_float * 64)()
 
