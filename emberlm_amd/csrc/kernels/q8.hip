@@ -231,6 +231,19 @@ int lanes_per_row(int64_t H) {
 
 constexpr int64_t kFewRows = 2048;
 
+// A launch holds fewer than 2^32 threads: a block per row, 2^24 of them, would not fit.
+constexpr int64_t kLaunchRows = int64_t{1} << 22;
+
+// run(first row, rows) for all rows, kLaunchRows at most at a time.
+template <typename Run>
+int by_launches(int64_t rows, Run run) {
+  for (int64_t r = 0; r < rows; r += kLaunchRows) {
+    run(r, rows - r < kLaunchRows ? rows - r : kLaunchRows);
+    if (const int rc = launch_status()) return rc;
+  }
+  return EMBER_OK;
+}
+
 // Blocks that quantise: several groups each, to keep the loads of some waves beside
 // the arithmetic of others.
 constexpr int64_t kQuantizeBlocks = 4096;
@@ -271,9 +284,11 @@ extern "C" int ember_q8_dequantize(const void* codes, const float* params, float
   auto launch = [&](auto lanes) {
     constexpr int LPR = decltype(lanes)::value;
     constexpr int RPB = kThreads / LPR;
-    q8_dequantize_kernel<LPR><<<static_cast<unsigned>((rows + RPB - 1) / RPB), kThreads, 0,
-                                as_stream(s)>>>(c, params, x, rows, H, ng);
-    return launch_status();
+    return by_launches(rows, [&](int64_t r, int64_t n) {
+      q8_dequantize_kernel<LPR><<<static_cast<unsigned>((n + RPB - 1) / RPB), kThreads, 0,
+                                  as_stream(s)>>>(c + r * row_bytes(H), params + 2 * r * ng,
+                                                  x + r * H, n, H, ng);
+    });
   };
   switch (lanes_per_row(H)) {
     case 8: return launch(std::integral_constant<int, 8>{});
@@ -292,18 +307,21 @@ extern "C" int ember_q8_dequantize_rmsnorm(const void* codes, const float* param
   if (!aligned16(codes) || !aligned8(params)) return EMBER_EALIGN;
   const auto* c = static_cast<const uint8_t*>(codes);
   const int64_t ng = row_groups(H);
-  if (rows < kFewRows || H > 4 * 64 * 16) {
-    q8_dequantize_rmsnorm_wide<<<static_cast<unsigned>(rows), kThreads, 0, as_stream(s)>>>(
-        c, params, w, x, y, rstd, H, ng, eps);
-    return launch_status();
-  }
+  if (rows < kFewRows || H > 4 * 64 * 16)
+    return by_launches(rows, [&](int64_t r, int64_t n) {
+      q8_dequantize_rmsnorm_wide<<<static_cast<unsigned>(n), kThreads, 0, as_stream(s)>>>(
+          c + r * row_bytes(H), params + 2 * r * ng, w, x + r * H, y + r * H,
+          rstd ? rstd + r : nullptr, H, ng, eps);
+    });
   auto launch = [&](auto lanes, auto pieces) {
     constexpr int LPR = decltype(lanes)::value, MAXC = decltype(pieces)::value;
     constexpr int RPB = kThreads / LPR;
-    q8_dequantize_rmsnorm_reg<LPR, MAXC>
-        <<<static_cast<unsigned>((rows + RPB - 1) / RPB), kThreads, 0, as_stream(s)>>>(
-            c, params, w, x, y, rstd, rows, static_cast<int>(H), static_cast<int>(ng), eps);
-    return launch_status();
+    return by_launches(rows, [&](int64_t r, int64_t n) {
+      q8_dequantize_rmsnorm_reg<LPR, MAXC>
+          <<<static_cast<unsigned>((n + RPB - 1) / RPB), kThreads, 0, as_stream(s)>>>(
+              c + r * row_bytes(H), params + 2 * r * ng, w, x + r * H, y + r * H,
+              rstd ? rstd + r : nullptr, n, static_cast<int>(H), static_cast<int>(ng), eps);
+    });
   };
   using std::integral_constant;
   switch (lanes_per_row(H)) {

@@ -447,3 +447,22 @@ def test_q8_rows_past_int32_offsets():
     v = OQ.values_rows8(ref_c, ref_p, H)
     close_roundings(host(x[-4:]), v)
     close_roundings(host(y[-4:]), v / np.sqrt((v * v).mean(1, keepdims=True)), H / 2 + 8)
+
+
+def test_q8_rows_of_more_than_one_launch():
+    rows, H = 2 ** 22 + 37, 8  # the second launch restores 37 rows
+    r = rng(5)
+    x = rows_like_keys(r, rows, H)
+    w = (1 + 0.1 * r.standard_normal(H)).astype(np.float32)
+    codes, params = quantised(x)
+    out, xo, y = (torch.full((rows, H), 5.0, device="cuda") for _ in range(3))
+    rstd, wd = torch.full((rows,), 5.0, device="cuda"), dev(w)
+    call("ember_q8_dequantize", p(codes), p(params), p(out), rows, H, None)
+    call("ember_q8_dequantize_rmsnorm", p(codes), p(params), p(wd), p(xo), p(y), p(rstd), rows, H,
+         1e-5, None)
+    assert torch.equal(out, xo)
+    v = OQ.values_rows8(*OQ.quantise_rows8(x), H)
+    close_roundings(host(xo), v)
+    ref = 1 / np.sqrt((v * v).mean(1) + 1e-5)
+    close_roundings(host(rstd), ref, (H + 5) / 2 + 2)  # as in test_q8_rows_and_their_norm
+    close_roundings(host(y), v * ref[:, None] * w, (H + 5) / 2 + 5)
