@@ -11,8 +11,8 @@
 // about one value in a million on the other side of a border between two
 // codes, and a value off by a whole step then looks like an error of the store.  A
 // wave forms it in fp32 first, whose error is below kNear, and again in fp64
-// only where some value of its lies that near a border (a wave in 16 of 255
-// steps, in 500 of 15): all in fp64, with two fp64 divisions a group,
+// only where some value of its lies that near a border (2 kNear of a wave's 512
+// values: a wave in 8 of 255 steps, in 140 of 15): all in fp64, with two fp64 divisions a group,
 // quantising 32768 x 2048 values took 90 us, so 67 (5.1 TB/s).
 #pragma once
 
