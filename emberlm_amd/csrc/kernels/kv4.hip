@@ -339,10 +339,12 @@ __device__ __forceinline__ void soften(const f32x4 (&s)[NT][2], const float* par
   for (int n = 0; n < NT; ++n) split_f16(x[n], hi[n], lo8[n]);
 }
 
-// A block's weights in pieces.  The references move, and the accumulators are
-// rescaled, only where some query's largest score passes its reference by more
-// than kMargin (the weights times steps then still fit in f16); that stands
-// outside of the two forms, or the compiler keeps two sets of accumulators.
+// A block's weights in pieces.  A query's reference moves, and its accumulators
+// are rescaled, only where its own largest score passes that reference by more
+// than kMargin (until then the weights times steps fit in f16): the other queries
+// of the wave keep theirs, to the bit, or a query's rounding would depend on keys
+// that only its neighbours see.  The rescaling stands outside of the two forms, or
+// the compiler keeps two sets of accumulators.
 // The wave goes first at the vector ALU while it is here: of two waves on a SIMD
 // one is then sooner back to feed the matrix core (1024 queries over 16384
 // keys 278 -> 259 us; first while it multiplies, 278).
@@ -363,8 +365,8 @@ __device__ __forceinline__ void softmax_block(bool mask, f32x4 (&s)[NT][2], cons
   if (__any(past)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float ref = fmaxf(st[n].ref, z[n]);
-      const float alpha = ref == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[n].ref - ref);
+      const float ref = z[n] > st[n].ref + kMargin ? z[n] : st[n].ref;
+      const float alpha = ref == st[n].ref ? 1.f : __builtin_amdgcn_exp2f(st[n].ref - ref);
       st[n].l *= alpha;
       st[n].olo *= alpha;
       st[n].ref = ref;

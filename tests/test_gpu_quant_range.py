@@ -1,0 +1,57 @@
+"""What a query's bits may depend on in the attention over a 4-bit cache."""
+import numpy as np
+import pytest
+
+from oracle import quant as OQ
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests.test_gpu_quant import attend, attention64, attention_bounds, same  # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    torch.cuda.init()
+
+
+def rng(s=0):
+    return np.random.default_rng(s)
+
+
+def held(x):
+    """A cache tensor's buffers and what it holds, of x [B, Hk, S, D]."""
+    codes, params = OQ.quantise(x.astype(np.float32), 15)
+    return OQ.pack4(codes), params, OQ.values(codes, params)
+
+
+# ------------------------------------------------------- a query and its neighbours
+@pytest.mark.parametrize("B,T,H,Hk,D,L", [
+    (1, 16, 2, 2, 128, 512),      # one workgroup of eight waves per head
+    (4, 16, 8, 8, 64, 4096),      # one query tile, key splits
+    (4, 16, 16, 8, 128, 4096),    # two
+    (1, 600, 1, 1, 64, 28000),    # shared tiles
+    (1, 600, 1, 1, 128, 28000),
+])
+def test_a_key_that_only_the_last_query_sees_moves_no_other_bit(B, T, H, Hk, D, L):
+    """Every query's scores rise by 3 (log2 units) among the last keys, less than lets its reference
+    move; the last key lifts the last query's score by a hundred, and that one's reference."""
+    r = rng(D + T)
+    d = r.standard_normal(D)
+    d /= np.linalg.norm(d)
+    q = (4 * d + 0.05 * r.standard_normal((B, T, H, D))).astype(np.float32)
+    rise = np.zeros(L)
+    rise[L - T:] = 3 * np.log(2) / 4
+    k = rise[:, None] * d + 0.02 * r.standard_normal((B, Hk, L, D))
+    v = held(r.standard_normal((B, Hk, L, D)))
+    quiet = attend(q, [held(k), v], L, L - T, 1.0)
+    k[:, :, L - 1] = 25 * d
+    loud = [held(k), v]
+    got = attend(q, loud, L, L - T, 1.0)
+    assert same(got[:, :-1], quiet[:, :-1])
+    ref = attention64(q, loud[0][2], v[2], L - T, 1.0, L)
+    worst, _ = attention_bounds(q, loud, 1.0, L)
+    assert np.abs(got - ref).max() <= worst
+    assert np.abs(got[:, -1] - quiet[:, -1]).max() > 0.1
