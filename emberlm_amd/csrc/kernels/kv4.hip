@@ -116,13 +116,15 @@ __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
 // where q' = q 2^(15 - ex) is a query scaled by a power of two so that its
 // largest element lies in [2^14, 2^15): its low pieces then stay normal f16.
 // The softmax runs against a reference per query
-//   ref ~ max_j (score_j + e_j - 8),  2^e_j > step of value row j,
+//   ref ~ max_j (score_j + e_j - 8),  2^e_j > step of value row j, 2^-40 |lo'_j|
 // instead of max score_j, so that the weights p_j = 2^(score_j - ref) times
 // their steps have their largest between 2^7 and 2^15 (ref may trail the
 // maximum by kMargin): the f16 range again, whatever the rows' sizes.  A weight
 // 2^-10 of the largest or more keeps its 22 bits, a smaller one is off by less
-// than 2^-32 of the largest.  e_j is at least -60, which bounds p_j by 2^75 where
-// steps vanish.  A query's bits depend on the rows it sees only.
+// than 2^-32 of the largest.  The offset's share in e_j bounds p_j |lo'_j| by
+// 2^55 where a row's step is small beside it or 0 (the codes' errors stay below
+// 2^-32 of the largest p |lo'| then); e_j is at least -60, which bounds p_j by
+// 2^75 where rows vanish.  A query's bits depend on the rows it sees only.
 //
 // Fragments (lane = (g = lane / 16, i = lane % 16)):
 //   S^T = K Q^T: A holds key i, dims g D/4 + 8 s + {0,4,1,5,2,6,3,7} in step s (the
@@ -141,6 +143,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlockKeys = 32;  // keys of one softmax step
 constexpr int kMinExp = -60, kShift = 8;
+constexpr float kLoPart = 0x1p-40f;
 constexpr float kMargin = 7.f;
 constexpr int kMaxSplits = 512;
 constexpr int64_t kMaxRows = 1 << 30;  // of a cache: row numbers are 32-bit in the kernels
@@ -270,7 +273,8 @@ __device__ __forceinline__ void stage_params(float* par, int key, bool value, fl
   par[(value ? kVStep : kKStep) * KEYS + key] = step;
   par[(value ? kVLo : kKLo) * KEYS + key] = lo8;
   if (value) {
-    const int ex = step > 0.f && !not_finite(step) ? __builtin_amdgcn_frexp_expf(step) : kMinExp;
+    const float size = fmaxf(step, fabsf(lo8) * kLoPart);
+    const int ex = size > 0.f && !not_finite(size) ? __builtin_amdgcn_frexp_expf(size) : kMinExp;
     par[kVExp * KEYS + key] = static_cast<float>((ex > kMinExp ? ex : kMinExp) - kShift);
   }
 }

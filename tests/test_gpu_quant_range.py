@@ -1,4 +1,4 @@
-"""What a query's bits may depend on in the attention over a 4-bit cache."""
+"""The attention over a 4-bit cache: what a query's bits may depend on, and value rows of any size."""
 import numpy as np
 import pytest
 
@@ -7,7 +7,8 @@ from oracle import quant as OQ
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from tests.test_gpu_quant import attend, attention64, attention_bounds, same  # noqa: E402
+from tests.test_gpu_quant import (attend, attention64, attention_bounds, check_attention,  # noqa: E402
+                                  same)
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -55,3 +56,23 @@ def test_a_key_that_only_the_last_query_sees_moves_no_other_bit(B, T, H, Hk, D, 
     worst, _ = attention_bounds(q, loud, 1.0, L)
     assert np.abs(got - ref).max() <= worst
     assert np.abs(got[:, -1] - quiet[:, -1]).max() > 0.1
+
+
+# ---------------------------------------------------------------- sizes of value rows
+def check_values(r, v, T, scale=None, Hk=2, G=2, D=64):
+    """Queries and keys of the usual size over the value rows v [1, Hk, L, D]."""
+    L = v.shape[2]
+    q = r.standard_normal((1, T, G * Hk, D)).astype(np.float32)
+    cache = [held(r.standard_normal((1, Hk, L, D))), held(v)]
+    return check_attention(q, cache, L, L - T, D ** -0.5 if scale is None else scale)
+
+
+@pytest.mark.parametrize("T,L", [(1, 1), (1, 300), (1, 3000), (20, 40), (70, 3000)])
+@pytest.mark.parametrize("power", [-100, -30, 20, 53, 60, 70, 99])
+def test_value_rows_of_equal_values(T, L, power):
+    """Rows without a step, held as they are: all of one size, and of sizes around it."""
+    r = rng(T + L)
+    v = np.ones((1, 2, L, 64)) * np.exp2(float(power))
+    check_values(r, v, T)
+    sign = r.choice([-1.0, 1.0], (1, 2, L, 1))
+    check_values(r, v * sign * np.exp2(-r.integers(0, 10, (1, 2, L, 1)).astype(float)), T)
