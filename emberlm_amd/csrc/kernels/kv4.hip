@@ -261,6 +261,18 @@ struct Softmax {
   float ref = -INFINITY, l = 0.f, olo = 0.f;
 };
 
+// References lie as far apart as e_j do, past the range of one exp2 where a row
+// of size 2^98 follows rows near 1, and the weights of these count in the sum all
+// the same: beyond 2^-kFar a weight sum is scaled in two factors.  Looked for
+// after the ordinary scaling, that costs 0.08 us (257 keys 5.27 -> 5.35; both
+// factors always, 5.65).  The outputs' sums need no such care: what 2^-126 takes
+// of them is below 2^-40 of the row that came.
+constexpr float kFar = 100.f;
+__device__ __forceinline__ float scale_far(float l, float d) {
+  return l * __builtin_amdgcn_exp2f(fmaxf(d, -kFar)) *
+         __builtin_amdgcn_exp2f(fminf(d + kFar, 0.f));
+}
+
 // The parameters of a block's keys in LDS, an array of KEYS floats each.
 enum { kKStep, kKLo, kVStep, kVLo, kVExp, kParams };
 
@@ -370,8 +382,10 @@ __device__ __forceinline__ void softmax_block(bool mask, f32x4 (&s)[NT][2], cons
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float ref = z[n] > st[n].ref + kMargin ? z[n] : st[n].ref;
-      const float alpha = ref == st[n].ref ? 1.f : __builtin_amdgcn_exp2f(st[n].ref - ref);
-      st[n].l *= alpha;
+      // nothing to rescale before the first
+      const float d = ref == st[n].ref || st[n].ref == -INFINITY ? 0.f : st[n].ref - ref;
+      const float alpha = __builtin_amdgcn_exp2f(d);
+      st[n].l = d < -kFar ? scale_far(st[n].l, d) : st[n].l * alpha;
       st[n].olo *= alpha;
       st[n].ref = ref;
 #pragma unroll
@@ -388,7 +402,11 @@ __device__ __forceinline__ void softmax_block(bool mask, f32x4 (&s)[NT][2], cons
 // The weight of a partial result with reference m and weight sum l against M.
 // Rows whose scores are all NaN leave m = -inf and l = NaN.
 __device__ __forceinline__ float merge_weight(float m, float l, float M) {
-  return m == -INFINITY ? (l == 0.f ? 0.f : l) : __builtin_amdgcn_exp2f(m - M);
+  return m == -INFINITY ? l : __builtin_amdgcn_exp2f(m - M);
+}
+// l brought from m to M where some partial result lies far from M.
+__device__ __forceinline__ float merge_far(float m, float l, float M) {
+  return m == -INFINITY ? l : scale_far(l, m - M);
 }
 
 // Block order: heads first, so that with 8 of them (or a multiple) a head's
@@ -731,12 +749,19 @@ __global__ __launch_bounds__(kWave * WAVES, 2) void attn_kv4_narrow(
     for (int v = 0; v < kWaves; ++v) M = fmaxf(M, sm[2 * (v * ROWS + row)]);
     float l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    bool far = false;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
       const int at = v * ROWS + row;
-      const float e = merge_weight(sm[2 * at], sm[2 * at + 1], M);
+      const float m = sm[2 * at], e = merge_weight(m, sm[2 * at + 1], M);
+      far |= m < M - kFar && m != -INFINITY;
       l += sm[2 * at + 1] * e;
       o += *reinterpret_cast<const f32x4*>(so + at * OS + 4 * c4) * e;
+    }
+    if (far) {
+      l = 0.f;
+      for (int v = 0; v < kWaves; ++v)
+        l += merge_far(sm[2 * (v * ROWS + row)], sm[2 * (v * ROWS + row) + 1], M);
     }
     const int64_t orow = attn_row(a, b, hk, r0 + row).row;
     if (a.nsplit == 1) {
@@ -945,8 +970,10 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
   }
   float l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  bool far = false;
   auto add = [&](int s, f32x4 v) {
-    const float ls = ml[2 * s + 1], e = merge_weight(ml[2 * s], ls, M);
+    const float m = ml[2 * s], ls = ml[2 * s + 1], e = merge_weight(m, ls, M);
+    far |= m < M - kFar && m != -INFINITY;
     l += ls * e;
     acc += v * e;
   };
@@ -956,6 +983,10 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
 #pragma unroll 4
   for (int s = part + kAhead * PARTS; s < nsplit; s += PARTS)
     add(s, *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(s) * D));
+  if (far) {
+    l = 0.f;
+    for (int s = part; s < nsplit; s += PARTS) l += merge_far(ml[2 * s], ml[2 * s + 1], M);
+  }
   s_o[threadIdx.x] = acc;
   s_l[threadIdx.x] = l;
   __syncthreads();

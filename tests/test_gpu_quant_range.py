@@ -76,3 +76,37 @@ def test_value_rows_of_equal_values(T, L, power):
     check_values(r, v, T)
     sign = r.choice([-1.0, 1.0], (1, 2, L, 1))
     check_values(r, v * sign * np.exp2(-r.integers(0, 10, (1, 2, L, 1)).astype(float)), T)
+
+
+@pytest.mark.parametrize("L", [256, 512, 4096])
+@pytest.mark.parametrize("T", [1, 3, 40])
+@pytest.mark.parametrize("first,last", [(0, 98), (98, 0), (-80, 98), (-90, 90), (-80, 50)])
+@pytest.mark.parametrize("equal", [True, False])
+def test_value_rows_of_two_sizes(T, L, first, last, equal):
+    """The first half of the keys (or every other run of 128) carries rows of one size, the rest of
+    another: the smaller ones count in the weights' sum as much as the larger."""
+    r = rng(T + L)
+    for large in (np.arange(L) >= L // 2, np.arange(L) // 128 % 2 == 1):
+        size = np.exp2(np.where(large, last, first).astype(float))[:, None]
+        v = r.standard_normal((1, 2, L, 64)) * size / 8
+        if equal:
+            small = ~large if first < last else large
+            v[:, :, small] = np.exp2(float(min(first, last)))
+        check_values(r, v, T, scale=0.05)
+
+
+@pytest.mark.parametrize("T", [600])
+@pytest.mark.parametrize("first,last", [(0, 98), (-80, 90)])
+def test_value_rows_of_two_sizes_shared_tiles(T, first, last):
+    r = rng(T)
+    L, D = 28000, 64
+    v = r.standard_normal((1, 1, L, D)) / 8
+    v[:, :, :L // 2] = 1
+    v *= np.exp2(np.where(np.arange(L) < L // 2, first, last).astype(float))[:, None]
+    q = r.standard_normal((1, T, 1, D)).astype(np.float32)
+    cache = [held(r.standard_normal((1, 1, L, D))), held(v)]
+    got = attend(q, cache, L, L - T, 0.05)
+    ref = attention64(q, cache[0][2], cache[1][2], L - T, 0.05, L)
+    worst, l2 = attention_bounds(q, cache, 0.05, L)
+    err = np.abs(got - ref)
+    assert err.max() <= worst and np.linalg.norm(err) <= l2 * np.linalg.norm(ref)
