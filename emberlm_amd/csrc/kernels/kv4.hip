@@ -123,8 +123,10 @@ __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
 // 2^-10 of the largest or more keeps its 22 bits, a smaller one is off by less
 // than 2^-32 of the largest.  The offset's share in e_j bounds p_j |lo'_j| by
 // 2^55 where a row's step is small beside it or 0 (the codes' errors stay below
-// 2^-32 of the largest p |lo'| then); e_j is at least -60, which bounds p_j by
-// 2^75 where rows vanish.  A query's bits depend on the rows it sees only.
+// 2^-32 of the largest p |lo'| then).  e_j is at least -80, which bounds p_j by
+// 2^95, and a sum of 2^30 of them by 2^125, where rows vanish; steps of 2^-90 still
+// keep 22 bits beside such a weight, and smaller ones are off by 2^-110 a row.
+// A query's bits depend on the rows it sees only.
 //
 // Fragments (lane = (g = lane / 16, i = lane % 16)):
 //   S^T = K Q^T: A holds key i, dims g D/4 + 8 s + {0,4,1,5,2,6,3,7} in step s (the
@@ -142,7 +144,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlockKeys = 32;  // keys of one softmax step
-constexpr int kMinExp = -60, kShift = 8;
+constexpr int kMinExp = -80, kShift = 8;
 constexpr float kLoPart = 0x1p-40f;
 constexpr float kMargin = 7.f;
 constexpr int kMaxSplits = 512;

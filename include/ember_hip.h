@@ -407,7 +407,9 @@ int ember_kv4_read_expanded(const uint32_t* codes, const float* params, float* o
  * visible one do not reach its output, whatever they hold.  D in {64, 128};
  * 1 <= L <= S <= 2^30, T and pos <= 2^30, fewer than 2^31 query rows and 2^23
  * workgroups (each takes 16 rows of a KV head at least, or all it has;
- * EMBER_EINVAL); magnitudes of keys and values below 2^100; alignment as above.  `workspace` >=
+ * EMBER_EINVAL); magnitudes of keys and values below 2^100 (rows of any sizes beside
+ * each other; a value row whose values span less than 2^-86 may be off by 2^-110
+ * where no larger row is seen); alignment as above.  `workspace` >=
  * ember_attn_kv4_workspace_bytes (0: none needed; EMBER_EWORKSPACE when
  * smaller) holds the partial results of key splits, merged in a fixed order:
  * deterministic. */

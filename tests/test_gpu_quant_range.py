@@ -110,3 +110,10 @@ def test_value_rows_of_two_sizes_shared_tiles(T, first, last):
     worst, l2 = attention_bounds(q, cache, 0.05, L)
     err = np.abs(got - ref)
     assert err.max() <= worst and np.linalg.norm(err) <= l2 * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("T,L", [(1, 1), (1, 300), (1, 3000), (20, 40), (70, 3000)])
+@pytest.mark.parametrize("power", [-80, -70, -61, 60, 96])
+def test_value_rows_all_of_one_size(T, L, power):
+    r = rng(T + L)
+    check_values(r, r.standard_normal((1, 2, L, 64)) * np.exp2(float(power)), T)
