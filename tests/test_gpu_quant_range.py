@@ -1,14 +1,18 @@
-"""The attention over a 4-bit cache: what a query's bits may depend on, and value rows of any size."""
+"""The attention over a 4-bit cache where values are very large, very small or all alike, what a
+query's bits may depend on, and the forms of the few-bit kernels that only large calls take."""
 import numpy as np
 import pytest
 
 from oracle import quant as OQ
+from tests.helpers import call, empty, host, p
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+from emberlm_amd import capi  # noqa: E402
 from tests.test_gpu_quant import (attend, attention64, attention_bounds, check_attention,  # noqa: E402
-                                  same)
+                                  close_roundings, held_cache, same)
+from tests.test_gpu_quant_model import test_decode_attention_kv4_fold as decode_step  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -117,3 +121,68 @@ def test_value_rows_of_two_sizes_shared_tiles(T, first, last):
 def test_value_rows_all_of_one_size(T, L, power):
     r = rng(T + L)
     check_values(r, r.standard_normal((1, 2, L, 64)) * np.exp2(float(power)), T)
+
+
+# ------------------------------------------------------------- forms of large calls
+@pytest.mark.parametrize("B,T,H,Hk,D,L,splits", [
+    (2, 1024, 32, 8, 64, 6000, 1),    # shared tiles, the output stored by themselves
+    (2, 2045, 16, 8, 128, 9003, 1),
+    (1, 8200, 16, 8, 128, 8200, 1),   # a whole prompt
+    (2, 1021, 16, 8, 128, 17003, 2),  # few splits, merged by a wave per row
+    (4, 16, 16, 8, 128, 300, 3),
+    (2, 64, 8, 4, 64, 900, 8),
+])
+def test_attention_of_few_or_no_key_splits(B, T, H, Hk, D, L, splits):
+    need = capi.lib().ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, L)
+    assert need == (0 if splits == 1 else B * T * H * splits * (D + 2) * 4)
+    r = rng(T)
+    q = r.standard_normal((B, T, H, D)).astype(np.float32)
+    cache = held_cache(r, B, Hk, L, D)
+    got = attend(q, cache, L, L - T, D ** -0.5)
+    ref = attention64(q, cache[0][2], cache[1][2], L - T, D ** -0.5, L)
+    worst, l2 = attention_bounds(q, cache, D ** -0.5, L)
+    err = np.abs(got - ref)
+    assert err.max() <= worst and np.linalg.norm(err) <= l2 * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("B,T,H,Hk,D,pos,S,qk,factor", [
+    (1, 1, 9, 3, 64, 700, 800, True, 0.0),     # heads of 64 over split keys
+    (2, 2, 8, 2, 64, 1027, 1030, False, 32.0),
+    (1, 1, 32, 8, 64, 6000, 6001, False, 0.0),
+])
+def test_decode_step_of_split_keys(B, T, H, Hk, D, pos, S, qk, factor):
+    assert capi.lib().ember_attn_kv4_workspace_bytes(B, T, H, Hk, D, pos + T) > 0
+    decode_step(B, T, H, Hk, D, pos, S, qk, factor)
+
+
+def test_kv4_write_and_read_of_more_rows_than_32_bits_number():
+    """2^31 + 10 head rows of 8 values written in one call, and read back as 2^32 + 20 pieces of
+    four.  Rows are checked at the ends, beside 2^31 and at random."""
+    torch.cuda.empty_cache()
+    T, Hk, D = 2 ** 30 + 5, 2, 8
+    rows = T * Hk
+    x = torch.empty(rows * D, device="cuda")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    for a in range(0, x.numel(), 2 ** 30):
+        x[a:a + 2 ** 30].normal_(generator=gen)
+    x = x.view(T, Hk, D)
+    kc, vc = (torch.zeros(rows, device="cuda", dtype=torch.int32) for _ in range(2))
+    kp, vp = (torch.zeros(rows * 2, device="cuda") for _ in range(2))
+    call("ember_kv4_write", p(x), p(x), p(kc), p(kp), p(vc), p(vp), 1, T, Hk, D, T, 0, None)
+    t = np.unique(np.concatenate([np.arange(40), 2 ** 29 + np.arange(-20, 20), T - 1 - np.arange(40),
+                                  rng(1).integers(0, T, 2000)]))
+    ti = torch.from_numpy(t).cuda()
+    codes, params = OQ.quantise(host(x[ti]).transpose(1, 0, 2), 15)
+    for c, par in ((kc, kp), (vc, vp)):
+        assert same(host(c.view(Hk, T)[:, ti]).view(np.uint32), OQ.pack4(codes)[..., 0])
+        assert same(host(par.view(Hk, T, 2)[:, ti]), params)
+    # every row of both tensors is written, and alike
+    assert torch.equal(kc, vc) and torch.equal(kp, vp)
+    assert bool((kp.view(-1, 2)[:, 1] > 0).all())
+    del x, vc, vp
+    out = empty((Hk, T, D))
+    call("ember_kv4_read_expanded", p(kc), p(kp), p(out), 1, Hk, 1, T, D, T, None)
+    close_roundings(host(out[:, ti]), OQ.values(codes, params))
+    del out, kc, kp
+    torch.cuda.empty_cache()
