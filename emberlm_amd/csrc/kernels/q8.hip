@@ -262,7 +262,7 @@ extern "C" size_t ember_q8_param_bytes(int64_t rows, int64_t H) {
 
 extern "C" int ember_q8_quantize(const float* x, void* codes, float* params, int64_t rows,
                                  int64_t H, ember_stream_t s) {
-  if (rows < 0 || H < 0) return EMBER_EINVAL;
+  if (rows < 0 || H < 0 || rows > 0x7fffffff) return EMBER_EINVAL;  // what can be restored
   if (rows == 0 || H == 0) return EMBER_OK;
   if (!x || !codes || !params) return EMBER_EINVAL;
   if (!aligned16(codes) || !aligned8(params)) return EMBER_EALIGN;

@@ -228,8 +228,8 @@ int ember_qknorm_rope_bwd(const float* dy, const float* x, const float* w, const
  * single values.
  * ember_q8_dequantize restores the rows; ember_q8_dequantize_rmsnorm also
  * gives y = x * rstd * w, the restored rows' RMSNorm (rstd[rows] may be NULL),
- * what a decoder block's re-run starts with; x and y must not overlap.  The two
- * restore fewer than 2^31 rows (EMBER_EINVAL). */
+ * what a decoder block's re-run starts with; x and y must not overlap.  All
+ * three take fewer than 2^31 rows (EMBER_EINVAL). */
 size_t ember_q8_code_bytes(int64_t rows, int64_t H);
 size_t ember_q8_param_bytes(int64_t rows, int64_t H);
 int ember_q8_quantize(const float* x, void* codes, float* params, int64_t rows, int64_t H,
