@@ -110,6 +110,15 @@ __device__ __forceinline__ float block_max(float v, float* smem) {
   return t;
 }
 
+// Whether the product of sizes (none negative) is a 64-bit number.
+template <typename... I>
+inline bool fits64(I... sizes) {
+  int64_t n = 1;
+  bool over = false;
+  ((over |= __builtin_mul_overflow(n, static_cast<int64_t>(sizes), &n)), ...);
+  return !over;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace ember

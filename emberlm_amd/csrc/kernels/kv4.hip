@@ -1055,6 +1055,12 @@ Plan attn_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t L) {
 // added to it.
 constexpr int64_t kIndex32 = int64_t{1} << 31;
 
+// The tensors' and the workspace's sizes in bytes are 64-bit numbers.
+bool attn_sizes_fit(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t S) {
+  return D <= kMaxRows && fits64(B, Hk, S, D, sizeof(float)) &&
+         fits64(B, T, H, D + 2, kMaxSplits, sizeof(float));
+}
+
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 }  // namespace
@@ -1064,7 +1070,8 @@ extern "C" int ember_kv4_write(const float* k, const float* v, uint32_t* k_codes
                                int64_t Hk, int64_t D, int64_t S, int64_t pos, ember_stream_t s) {
   if (B < 0 || T < 0 || Hk < 0 || pos < 0 || T > S || pos > S - T) return EMBER_EINVAL;
   if (D < 8 || D > kMaxD || D % 8) return EMBER_EINVAL;
-  if (B * T * Hk == 0) return EMBER_OK;
+  if (B == 0 || T == 0 || Hk == 0) return EMBER_OK;
+  if (!fits64(B, Hk, S, D, sizeof(float))) return EMBER_EINVAL;
   if (!k || !v || !k_codes || !k_params || !v_codes || !v_params) return EMBER_EINVAL;
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_codes) || !aligned16(v_codes) ||
       !aligned8(k_params) || !aligned8(v_params))
@@ -1093,8 +1100,10 @@ extern "C" int ember_kv4_read_expanded(const uint32_t* codes, const float* param
                                        int64_t S, ember_stream_t s) {
   if (B < 0 || Hk < 0 || group <= 0 || L < 0 || L > S) return EMBER_EINVAL;
   if (D < 8 || D > kMaxD || D % 8) return EMBER_EINVAL;
+  if (B == 0 || Hk == 0 || L == 0) return EMBER_OK;
+  if (!fits64(B, Hk, S, D, sizeof(float)) || !fits64(B, Hk, L, D, group, sizeof(float)))
+    return EMBER_EINVAL;
   const int64_t n = B * Hk * L * (D / 4);
-  if (n == 0) return EMBER_OK;
   if (!codes || !params || !out) return EMBER_EINVAL;
   if (!aligned16(codes) || !aligned16(out) || !aligned8(params)) return EMBER_EALIGN;
   const unsigned grid = grid_1d(n, kThreads);
@@ -1110,7 +1119,9 @@ extern "C" int ember_kv4_read_expanded(const uint32_t* codes, const float* param
 
 extern "C" size_t ember_attn_kv4_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk,
                                                  int64_t D, int64_t L) {
-  if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || L <= 0) return 0;
+  if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || L <= 0 ||
+      !attn_sizes_fit(B, T, H, Hk, D, L))
+    return 0;
   const Plan p = attn_plan(B, T, H, Hk, L);
   if (p.nsplit == 1) return 0;
   return static_cast<size_t>(B * T * H) * p.nsplit * (D + 2) * sizeof(float);
@@ -1193,6 +1204,7 @@ extern "C" int ember_attn_kv4(const float* q, const uint32_t* k_codes, const flo
   if (D != 64 && D != 128) return EMBER_EINVAL;
   if (B == 0 || T == 0) return EMBER_OK;
   if (L < 1 || L > S || S > kMaxRows || T > kMaxRows || pos > kMaxRows) return EMBER_EINVAL;
+  if (!attn_sizes_fit(B, T, H, Hk, D, S)) return EMBER_EINVAL;
   if (!q || !k_codes || !k_params || !v_codes || !v_params || !o) return EMBER_EINVAL;
   if (!aligned16(q) || !aligned16(o) || !aligned16(k_codes) || !aligned16(v_codes) ||
       !aligned8(k_params) || !aligned8(v_params))
@@ -1214,6 +1226,7 @@ extern "C" int ember_attn_kv4_qkv(const float* q, const float* k, const float* v
     return EMBER_EINVAL;
   if (S > kMaxRows || T > S || pos > S - T) return EMBER_EINVAL;
   if (B == 0 || T == 0) return EMBER_OK;
+  if (!attn_sizes_fit(B, T, H, Hk, D, S)) return EMBER_EINVAL;
   if (!q || !k || !v || !o || !k_codes || !k_params || !v_codes || !v_params) return EMBER_EINVAL;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(k_codes) ||
       !aligned16(v_codes) || !aligned8(k_params) || !aligned8(v_params) ||

@@ -248,22 +248,30 @@ int by_launches(int64_t rows, Run run) {
 // the arithmetic of others.
 constexpr int64_t kQuantizeBlocks = 4096;
 
+// The rows' size in bytes, and that of their codes and pairs, are 64-bit numbers.
+bool sizes_fit(int64_t rows, int64_t H) {
+  return H <= INT64_MAX / 32 && fits64(rows, H + 16, sizeof(float));
+}
+
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 }  // namespace
 
 extern "C" size_t ember_q8_code_bytes(int64_t rows, int64_t H) {
-  return rows > 0 && H > 0 ? static_cast<size_t>(rows * row_bytes(H)) : 0;
+  return rows > 0 && H > 0 && sizes_fit(rows, H) ? static_cast<size_t>(rows * row_bytes(H)) : 0;
 }
 
 extern "C" size_t ember_q8_param_bytes(int64_t rows, int64_t H) {
-  return rows > 0 && H > 0 ? static_cast<size_t>(rows * row_groups(H)) * 2 * sizeof(float) : 0;
+  return rows > 0 && H > 0 && sizes_fit(rows, H)
+             ? static_cast<size_t>(rows * row_groups(H)) * 2 * sizeof(float)
+             : 0;
 }
 
 extern "C" int ember_q8_quantize(const float* x, void* codes, float* params, int64_t rows,
                                  int64_t H, ember_stream_t s) {
   if (rows < 0 || H < 0 || rows > 0x7fffffff) return EMBER_EINVAL;  // what can be restored
   if (rows == 0 || H == 0) return EMBER_OK;
+  if (!sizes_fit(rows, H)) return EMBER_EINVAL;
   if (!x || !codes || !params) return EMBER_EINVAL;
   if (!aligned16(codes) || !aligned8(params)) return EMBER_EALIGN;
   const int64_t ng = row_groups(H);
@@ -277,6 +285,7 @@ extern "C" int ember_q8_dequantize(const void* codes, const float* params, float
                                    int64_t H, ember_stream_t s) {
   if (rows < 0 || H < 0 || rows > 0x7fffffff) return EMBER_EINVAL;
   if (rows == 0 || H == 0) return EMBER_OK;
+  if (!sizes_fit(rows, H)) return EMBER_EINVAL;
   if (!x || !codes || !params) return EMBER_EINVAL;
   if (!aligned16(codes) || !aligned8(params)) return EMBER_EALIGN;
   const auto* c = static_cast<const uint8_t*>(codes);
@@ -303,6 +312,7 @@ extern "C" int ember_q8_dequantize_rmsnorm(const void* codes, const float* param
                                            int64_t H, float eps, ember_stream_t s) {
   if (rows < 0 || H < 0 || rows > 0x7fffffff) return EMBER_EINVAL;
   if (rows == 0 || H == 0) return EMBER_OK;
+  if (!sizes_fit(rows, H)) return EMBER_EINVAL;
   if (!x || !y || !w || !codes || !params) return EMBER_EINVAL;
   if (!aligned16(codes) || !aligned8(params)) return EMBER_EALIGN;
   const auto* c = static_cast<const uint8_t*>(codes);
