@@ -84,9 +84,10 @@ Request parse_request(const std::string& text) {
   if (const JVal* v = req.find("think_open_ids")) r.think_open_ids = ids(*v, "think_open_ids");
   if (const JVal* v = req.find("think_close_ids")) r.think_close_ids = ids(*v, "think_close_ids");
   if (const JVal* v = req.find("kv_bits")) {
-    r.kv_bits = static_cast<int>(integer(*v, "kv_bits"));
-    if (r.kv_bits != 32 && r.kv_bits != 4)
+    const int64_t bits = integer(*v, "kv_bits");
+    if ((bits != 32 && bits != 4) || v->num != static_cast<double>(bits))  // 4.5 is not 4
       throw std::runtime_error("request: kv_bits must be 32 or 4");
+    r.kv_bits = static_cast<int>(bits);
   }
   return r;
 }

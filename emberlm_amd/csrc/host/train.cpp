@@ -152,9 +152,12 @@ Config load_config(const fs::path& cfg_path) {
   }
   c.offload_optimizer = get_bool(j, "offload_optimizer", c.offload_optimizer);
   c.gradient_checkpointing = get_bool(j, "gradient_checkpointing", c.gradient_checkpointing);
-  c.checkpoint_bits = get_int(j, "checkpoint_bits", c.checkpoint_bits);
-  if (c.checkpoint_bits != 32 && (c.checkpoint_bits != 8 || !c.gradient_checkpointing))
-    throw std::runtime_error("config: checkpoint_bits must be 32, or 8 with gradient_checkpointing");
+  if (const json::JVal* b = key(j, "checkpoint_bits")) {
+    if (b->kind != json::JVal::kNum || (b->num != 32 && (b->num != 8 || !c.gradient_checkpointing)))
+      throw std::runtime_error(
+          "config: checkpoint_bits must be 32, or 8 with gradient_checkpointing");
+    c.checkpoint_bits = static_cast<int>(b->num);
+  }
   if (const json::JVal* m = key(j, "model")) {
     c.model = model_config(*m);
     c.has_model = true;

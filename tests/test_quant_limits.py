@@ -1,8 +1,14 @@
 """CPU checks of what the few-bit stores' entry points refuse: sizes that one of a pair of calls
 would take and the other not, that pass 64 bits, and bits that are not whole numbers."""
 import ctypes as C
+import json
+import os
+import subprocess
+
+import pytest
 
 from emberlm_amd import capi
+from emberlm_amd import trainer as TR
 
 P = C.c_void_p(4096)  # never dereferenced
 
@@ -51,3 +57,31 @@ def test_sizes_that_pass_64_bits():
     # nothing to do is still nothing to do, whatever the other sizes
     assert write(0, 1, 8, 2 ** 62) == 0 and read(0, 1, 1, 1, 2 ** 62) == 0
     assert lib.ember_q8_quantize(P, P, P, 0, 2 ** 63 - 1, None) == 0
+
+
+@pytest.mark.parametrize("bits", ["4.5", "32.25", str(2 ** 32 + 4), "-4", "0"])
+def test_kv_bits_are_32_or_4_and_nothing_that_rounds_to_them(bits):
+    exe = os.path.join(os.path.dirname(TR.LIB_PATH), "ctd_generate")
+    r = subprocess.run([exe, "--model", "/nonexistent.safetensors"],
+                       input='{"input_ids": [1], "kv_bits": %s}' % bits, capture_output=True,
+                       text=True, timeout=60)
+    assert r.returncode == 1 and "kv_bits must be 32 or 4" in json.loads(r.stdout)["error"]
+
+
+@pytest.mark.parametrize("bits", ["8.5", "32.25", str(2 ** 32 + 8), "-8", '"8"'])
+def test_checkpoint_bits_are_32_or_8_and_nothing_that_rounds_to_them(tmp_path, bits):
+    cfg = tmp_path / "config.json"
+    cfg.write_text('{"init_weights": "w", "data_dir": "d", "gradient_checkpointing": true, '
+                   '"checkpoint_bits": %s}' % bits)
+    with pytest.raises(TR.CtdError, match="checkpoint_bits must be 32, or 8"):
+        TR.train_run(cfg)
+
+
+@pytest.mark.parametrize("bits", ["32", "4", "4.0", "3.2e1"])
+def test_kv_bits_that_are_taken(bits):
+    """The request passes; what fails then is the model file."""
+    exe = os.path.join(os.path.dirname(TR.LIB_PATH), "ctd_generate")
+    r = subprocess.run([exe, "--model", "/nonexistent.safetensors"],
+                       input='{"input_ids": [1], "kv_bits": %s}' % bits, capture_output=True,
+                       text=True, timeout=60)
+    assert r.returncode == 1 and "kv_bits" not in json.loads(r.stdout)["error"]
