@@ -126,6 +126,10 @@ __global__ __launch_bounds__(kThreads) void kv4_read_expanded_kernel(
 // 2^-32 of the largest p |lo'| then).  e_j is at least -80, which bounds p_j by
 // 2^95, and a sum of 2^30 of them by 2^125, where rows vanish; steps of 2^-90 still
 // keep 22 bits beside such a weight, and smaller ones are off by 2^-110 a row.
+// Scores reach 2^22 log2 units: the roundings of score_j + e_j - 8, in ref and
+// beside it, are then at most 1/8 each, so weights times steps stay below 2^15.25,
+// and f16 ends at 2^16 (scores rounded before ref is taken from them would have no
+// such end, for one instruction more each).
 // A query's bits depend on the rows it sees only.
 //
 // Fragments (lane = (g = lane / 16, i = lane % 16)):

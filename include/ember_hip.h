@@ -409,7 +409,9 @@ int ember_kv4_read_expanded(const uint32_t* codes, const float* params, float* o
  * workgroups (each takes 16 rows of a KV head at least, or all it has;
  * EMBER_EINVAL); magnitudes of keys and values below 2^100 (rows of any sizes beside
  * each other; a value row whose values span less than 2^-86 may be off by 2^-110
- * where no larger row is seen); alignment as above.  `workspace` >=
+ * where no larger row is seen) and scores |scale q . k| below 2^21, beyond which
+ * their own fp32 rounding may reach the outputs as Inf or NaN; alignment as above.
+ * `workspace` >=
  * ember_attn_kv4_workspace_bytes (0: none needed; EMBER_EWORKSPACE when
  * smaller) holds the partial results of key splits, merged in a fixed order:
  * deterministic. */

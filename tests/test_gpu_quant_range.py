@@ -123,6 +123,39 @@ def test_value_rows_all_of_one_size(T, L, power):
     check_values(r, r.standard_normal((1, 2, L, 64)) * np.exp2(float(power)), T)
 
 
+@pytest.mark.parametrize("T,L", [(1, 1), (1, 300), (1, 4096), (20, 40), (16, 512), (70, 3000)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_near_the_largest_that_are_taken(T, L, D, sign):
+    """Scores up to 2^21 in steps of some hundreds: each query's output is the value row of its
+    largest score, to the weights' 22 bits and the sums' roundings.  Value rows differ in size."""
+    r = rng(T + L)
+    B, H, Hk = 1, 4, 2
+    q = np.abs(r.standard_normal((B, T, H, D))) + 0.5
+    k = np.ones((B, Hk, L, D)) + 0.001 * r.standard_normal((B, Hk, L, D))
+    level = np.stack([r.permutation(L) for _ in range(Hk)]).reshape(B, Hk, L, 1)
+    k *= 1 + level / L  # the order of a query's scores is that of the levels
+    q, cache = q.astype(np.float32), [held(k), None]
+    v = r.standard_normal((B, Hk, L, D)) * np.exp2(r.integers(-40, 40, (B, Hk, L, 1)).astype(float))
+    cache[1] = held(v)
+    top = np.einsum("bthd,bhld->bthl", q.astype(np.float64).reshape(B, T, Hk * 2, D),
+                    np.repeat(cache[0][2], 2, 1)).max()
+    scale = sign * 0.99 * 2.0 ** 21 / top
+    got = attend(q, cache, L, L - T, scale)
+    for t in range(T):
+        n = L - T + t + 1
+        for h in range(H):
+            kk, vv = cache[0][2][0, h // 2, :n], cache[1][2][0, h // 2, :n]
+            s = kk @ q[0, t, h].astype(np.float64) * scale
+            j = s.argmax()
+            others = np.delete(s, j)
+            if others.size and s[j] - others.max() < 120:  # not this one's alone
+                continue
+            tol = (2.0 ** -22 + 30 * 2.0 ** -24) * (np.abs(vv[j]).max() + 16 * cache[1][1][0, h // 2, j, 1])
+            assert np.abs(got[0, t, h] - vv[j]).max() <= tol, (t, h, j)
+    assert np.isfinite(got).all()
+
+
 # ------------------------------------------------------------- forms of large calls
 @pytest.mark.parametrize("B,T,H,Hk,D,L,splits", [
     (2, 1024, 32, 8, 64, 6000, 1),    # shared tiles, the output stored by themselves
