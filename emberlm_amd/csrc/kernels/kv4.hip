@@ -175,8 +175,10 @@ __device__ __forceinline__ f32x4 mfma(half8_t a, half8_t b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// The eight codes of a word, less 8, in the order 0 4 1 5 2 6 3 7: bits of f16
-// 1024 + c and 1024 + 16 c, then exact arithmetic.  `one` is 0x64006400 (two
+// The eight codes of a word, less 8, in the order 0 4 1 5 2 6 3 7, by the known
+// way from small integers to floats: a code or-ed into the mantissa of 1024 makes
+// 1024 + c (or + 16 c, where it lies four bits up), and what was added comes off
+// again exactly.  `one` is 0x64006400 (two
 // f16 1024) in a register of its own: a mask and an or of two literals would be
 // two instructions.
 __device__ __forceinline__ uint32_t two_1024() {
@@ -554,13 +556,15 @@ __device__ __forceinline__ void fold_rows(const AttnArgs& a, const Fold& f,
 // codes and are merged through LDS.  The next block's loads (five or so per
 // lane: K as fragments, V as 16-byte pieces that pass through LDS for their
 // transpose, one pair of parameters) are in flight during a block.  One token at
-// 130001 keys, 8 KV heads of 128: 33 us, 4.6 TB/s, the vector ALU busy 64% of them.
+// 130001 keys, 8 KV heads of 128: 32 us, 4.7 TB/s, the vector ALU busy 55% of them.
 //
 // FOLD: a decode step's raw projections.  Queries are normalised and rotated as
 // they are loaded, and the workgroup whose blocks hold the new rows quantises
 // them into the cache before it reads any of its blocks; no other workgroup
 // of that head reads them, except those of another row tile, which write the
-// same bits themselves.
+// same bits themselves.  Sines, the new rows and two barriers before the owner's
+// first load make 2 to 3 us: 257 keys 7.5 against 5.2, 4096 keys 9.2 against 6.4,
+// 130001 keys 34.5 against 31.9.
 template <int D, int NT, int WAVES, bool FOLD>
 __global__ __launch_bounds__(kWave * WAVES, 2) void attn_kv4_narrow(
     AttnArgs a, std::conditional_t<FOLD, Fold, NoFold> f) {
@@ -787,8 +791,8 @@ __global__ __launch_bounds__(kWave * WAVES, 2) void attn_kv4_narrow(
 // that hold them as fragments, 16 bytes per lane one after another, so that
 // every wave's reads are free of bank conflicts; the next tile's codes are
 // loaded during a tile and unpacked after it.  1024 queries at 16384 keys, 16
-// heads of 128: 243 us and 9 for the merge, 530 TFLOP/s (twice that on the matrix
-// cores); bound by the vector ALU and the matrix cores, which two waves of a
+// heads of 128: 243 us, and 9 for the merge: 530 TFLOP/s in all (twice that on the
+// matrix cores); bound by the vector ALU and the matrix cores, which two waves of a
 // SIMD keep busy at once for about half of the time.
 constexpr int kWideRows = 128;
 constexpr int kTileKeys = 64;
@@ -939,7 +943,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_kv4_wide(AttnArgs a) {
 // Merges a row's splits in a fixed order.  PARTS groups of D/4 lanes take every
 // PARTS-th split of a row each, four at a time, and are then added in order:
 // a wave per row (PARTS = 256 / D) where splits are few, a block per row (1024 / D)
-// where they are many (a token at 4096 keys, 32 splits: 7.75 against 8.95 us in
+// where they are many (a token at 4096 keys, 32 splits: 7.9 against 9.2 us in
 // all).
 template <int D, int PARTS>
 __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __restrict__ part_o,
@@ -1010,18 +1014,18 @@ __global__ __launch_bounds__(kThreads) void attn_kv4_combine(const float* __rest
 // an MI355X).
 //  - R <= 16, a decode step: one query tile.  Up to kOneKeys keys, or where every
 //    CU has a head of its own, one workgroup of eight waves per head and no second
-//    launch (257 keys 5.2 against 6.4 in splits of four waves, 512 keys 7.6 and
-//    7.3, 1024 keys 8.6 and 7.3; 256 heads of 4000 keys 33.9 and 36.0); else splits.
+//    launch (257 keys 6.5 against 7.1 in splits of four waves, 512 keys 7.5 and
+//    7.3, 1024 keys 10.4 and 7.3; 256 heads of 4000 keys 33.6 and 36.0); else splits.
 //  - beyond, two query tiles, each workgroup for itself; or the shared tiles of
 //    128 rows where there is so much to do that unpacking counts for more than
-//    their barriers, kWideWork rows times keys or more (512 rows: 16384 keys 92
-//    against 94, 32768 keys 165 and 156; 2048 rows: 4096 keys 78 and 84, 16384
-//    keys 303 and 281).
+//    their barriers, kWideWork rows times keys or more (512 rows: 16384 keys 102
+//    against 101, 32768 keys 176 and 161; 2048 rows: 4096 keys 85 and 91, 16384
+//    keys 308 and 278).
 //  - Splits: a workgroup for each CU, two where that leaves kLongKeys keys or more
-//    to each (130001 keys 36 against 42 with one; 4096 keys and 128 rows, where
+//    to each (130001 keys 36 against 43 with one; 4096 keys and 128 rows, where
 //    the partial results weigh more, 23 against 19), and 32 keys a wave at least.
 //    A prompt whose row tiles fill the GPU once, the later ones with twice the
-//    mean's keys, is split in two all the same (4096 queries and keys 220 -> 176).
+//    mean's keys, is split in two all the same (4096 queries and keys 235 -> 194).
 constexpr int64_t kCus = 256;
 constexpr int64_t kOneKeys = 512;
 constexpr int64_t kWideWork = int64_t{1} << 24;

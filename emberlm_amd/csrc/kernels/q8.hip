@@ -138,9 +138,9 @@ __global__ __launch_bounds__(kThreads) void q8_dequantize_kernel(
 }
 
 // The restored rows and their RMSNorm, the row held in registers between the
-// two: LPR lanes, MAXC pieces of four columns each.  32768 x 2048: 135 us, 4.5
+// two: LPR lanes, MAXC pieces of four columns each.  32768 x 2048: 130 us, 4.7
 // TB/s (a large copy reaches 5.2); a block per row that reads the codes twice
-// takes 142.
+// takes 7 more.
 template <int LPR, int MAXC>
 __global__ __launch_bounds__(kThreads) void q8_dequantize_rmsnorm_reg(
     const uint8_t* __restrict__ codes, const float* __restrict__ params,
@@ -193,7 +193,8 @@ __global__ __launch_bounds__(kThreads) void q8_dequantize_rmsnorm_reg(
 
 // The same a block per row, the codes read twice: for rows of any width, and
 // for so few rows that a wave each would leave most of the GPU idle (511 x 576:
-// 3.8 against 4.9 us).
+// 3.7 against 3.9 us, 300 x 2048: 4.8 against 6.1; at 1500 x 2048 already 9.2
+// against 8.6, at 2048 x 2048 11.8 both).
 __global__ __launch_bounds__(kThreads) void q8_dequantize_rmsnorm_wide(
     const uint8_t* __restrict__ codes, const float* __restrict__ params,
     const float* __restrict__ w, float* __restrict__ x, float* __restrict__ y,

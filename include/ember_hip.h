@@ -224,8 +224,8 @@ int ember_qknorm_rope_bwd(const float* dy, const float* x, const float* w, const
  * codes: rows of round_up(H, 16) bytes, the padding 0; params
  * [rows][ceil(H/128)][2]; their sizes are ember_q8_code_bytes and
  * ember_q8_param_bytes.  Any H; codes 16-byte and params 8-byte aligned
- * (EMBER_EALIGN); fp32 rows that are not 16-byte aligned are accessed by
- * single values.
+ * (EMBER_EALIGN); fp32 rows may start at any float, and are accessed four
+ * values at a time there too (a row's last one to three singly).
  * ember_q8_dequantize restores the rows; ember_q8_dequantize_rmsnorm also
  * gives y = x * rstd * w, the restored rows' RMSNorm (rstd[rows] may be NULL),
  * what a decoder block's re-run starts with; x and y must not overlap.  All
