@@ -127,6 +127,15 @@ SIGNATURES = {
     "ember_q8_quantize": (i32, [vp, vp, vp, i64, i64, vp]),
     "ember_q8_dequantize": (i32, [vp, vp, vp, i64, i64, vp]),
     "ember_q8_dequantize_rmsnorm": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, f32, vp]),
+    "ember_mx4_code_bytes": (sz, [i64, i64]),
+    "ember_mx4_scale_bytes": (sz, [i64, i64]),
+    "ember_mx4_quantize": (i32, [vp, vp, vp, i64, i64, vp]),
+    "ember_mx4_dequantize": (i32, [vp, vp, vp, i64, i64, vp]),
+    "ember_mx4_embedding": (i32, [vp, vp, vp, vp, i64, i64, i64, vp]),
+    "ember_mx4_workspace_bytes": (sz, [i64, i64, i64]),
+    "ember_mx4_linear": (i32, [vp, i64, i64, vp, f32, i32, C.POINTER(vp), C.POINTER(vp),
+                               C.POINTER(i64), C.POINTER(vp), C.POINTER(vp), vp, sz, vp]),
+    "ember_mx4_gateup": (i32, [vp, i64, i64, vp, f32, vp, vp, vp, vp, i64, vp, vp, sz, vp]),
     "ember_argmax_rows": (i32, [vp, i64, i64, vp, vp]),
     "ember_argmax_rows_workspace_bytes": (sz, [i64, i64]),
     "ember_argmax_rows_ws": (i32, [vp, i64, i64, vp, vp, sz, vp]),

@@ -436,6 +436,56 @@ int ember_attn_kv4_qkv(const float* q, const float* k, const float* v, int64_t B
                        int64_t S, float scale, float* o, void* workspace, size_t workspace_bytes,
                        ember_stream_t s);
 
+/* ------------------------------------------------------ weights in 4 bits
+ * Added in this build (the reference's weights are fp32).  A weight [N, K] in
+ * microscaled 4-bit floating point: each row in groups of 32 values (the last
+ * may be shorter), a group's scale one byte b, 2^(b - 127), and per value a
+ * code of four bits, a sign above the index of its size in {0, 1/2, 1, 3/2, 2, 3,
+ * 4, 6}; code times scale is the value.  The scale is the smallest power of two
+ * (2^-127 at least) that the group's largest size is at most 7 times of; a
+ * value takes the size nearest to its quotient by it, of two as near the one of
+ * even index, above 6 always 6.  A group with an infinity or a NaN reads back as
+ * NaN throughout (b = 255).  Magnitudes below 2^127.
+ * Two buffers hold it, of ember_mx4_code_bytes and ember_mx4_scale_bytes, 16-byte
+ * aligned (EMBER_EALIGN): tiles of 32 rows by 64 columns, 1024 bytes each, a row
+ * of tiles after another, byte 16 (32 h + r) + i of a tile holding columns 32 h +
+ * 2 i (low half) and 32 h + 2 i + 1 of its row r; and blocks of 256 scales for 32
+ * rows by 256 columns, byte 4 (32 h + r) + c for columns 64 c + 32 h and up of
+ * row r.  What fills up the last tiles is 0.  1 <= K <= 2^30, N < 2^31
+ * (EMBER_EINVAL; the sizes are then 0).  fp32 rows may start at any float.
+ *
+ * ember_mx4_quantize brings w [N, K] into that form, ember_mx4_dequantize reads
+ * it back, and ember_mx4_embedding gives rows of it: out [n, K], row i = row
+ * ids[i], zeros for ids outside [0, V); fewer than 2^31 ids. */
+size_t ember_mx4_code_bytes(int64_t N, int64_t K);
+size_t ember_mx4_scale_bytes(int64_t N, int64_t K);
+int ember_mx4_quantize(const float* w, void* codes, void* scales, int64_t N, int64_t K,
+                       ember_stream_t s);
+int ember_mx4_dequantize(const void* codes, const void* scales, float* w, int64_t N, int64_t K,
+                         ember_stream_t s);
+int ember_mx4_embedding(const int64_t* ids, const void* codes, const void* scales, float* out,
+                        int64_t n, int64_t K, int64_t V, ember_stream_t s);
+/* Products with such weights, for any number of rows M < 2^31 of x [M, K]
+ * (any float's address; K as above; at least one row each in the weights).
+ * ember_mx4_linear: for i < nseg (1..3), y[i] [M, N[i]] = xn W_i^T
+ * (+ residual[i] [M, N[i]] where residual and residual[i] are not NULL; y[i] may be
+ * residual[i]), xn = x where norm_w is NULL, else RMSNorm(x) with weight
+ * norm_w [K] and eps.  ember_mx4_gateup: out [M, I] = silu(xn Wg^T) * (xn Wu^T).
+ * The codes enter the products as they are held; sums are fp32.  A row of x that
+ * is not finite throughout gives a row that is finite nowhere.
+ * `workspace` >= ember_mx4_workspace_bytes(M, K, rows of all the call's weights)
+ * (0: none needed; EMBER_EWORKSPACE when smaller), 256-byte aligned (EMBER_EALIGN).
+ * Host arrays are read at the call.  Deterministic. */
+size_t ember_mx4_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int ember_mx4_linear(const float* x, int64_t M, int64_t K, const float* norm_w, float eps,
+                     int nseg, const void* const* codes, const void* const* scales,
+                     const int64_t* N, float* const* y, const float* const* residual,
+                     void* workspace, size_t workspace_bytes, ember_stream_t s);
+int ember_mx4_gateup(const float* x, int64_t M, int64_t K, const float* norm_w, float eps,
+                     const void* gate_codes, const void* gate_scales, const void* up_codes,
+                     const void* up_scales, int64_t I, float* out, void* workspace,
+                     size_t workspace_bytes, ember_stream_t s);
+
 /* ------------------------------------------------------ fused decode step
  * Kernels for calls of at most 8 token rows (decode), each streaming its
  * weights once with the small ops around it folded in.  No counterpart kernel
