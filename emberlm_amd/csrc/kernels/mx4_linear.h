@@ -1,0 +1,54 @@
+// What the entry points of the products with 4-bit weights (mx4_linear.hip)
+// share with their kernels.
+#pragma once
+
+#include <cmath>
+
+#include "mx4.h"
+
+namespace ember {
+
+constexpr int kMx4MaxSeg = 3;  // weights of one ember_mx4_linear call
+
+struct Mx4Weight {
+  const uint32_t* codes;
+  const uint32_t* scales;
+};
+
+// One call's products.  SwiGLU (gate): weights 0 and 1 are the gate's and the
+// up projection's, both of N[0] rows, y[0] the output.
+struct Mx4Call {
+  const float* x;
+  const float* norm_w;  // NULL: x as it is
+  float eps;
+  int64_t M, K;
+  int64_t kb, ks;  // tiles and scale blocks along K
+  Mx4Weight W[kMx4MaxSeg];
+  const float* res[kMx4MaxSeg];
+  float* y[kMx4MaxSeg];
+  int64_t N[kMx4MaxSeg];
+  int nseg;
+  bool x_vec;  // rows of x and the norm's weight are whole aligned float4s
+};
+
+// The segment and its block of a workgroup that takes block b of all segments'
+// column blocks (first[i]: the first of segment i).
+struct Mx4Blocks {
+  int64_t first[kMx4MaxSeg + 1];
+};
+__device__ __forceinline__ int mx4_segment(const Mx4Blocks& bl, int nseg, int64_t& b) {
+  int seg = 0;
+  while (seg + 1 < nseg && b >= bl.first[seg + 1]) ++seg;
+  b -= bl.first[seg];
+  return seg;
+}
+
+__device__ __forceinline__ float mx4_silu_mul(float g, float u) {
+  return g * (1.0f / (1.0f + expf(-g))) * u;
+}
+
+// Calls of at most kMx4FewRows rows (mx4_few.hip).
+constexpr int kMx4FewRows = 8;
+int mx4_few_rows(const Mx4Call& c, bool gate, hipStream_t st);
+
+}  // namespace ember

@@ -2,33 +2,11 @@
 // mx4.h): y = W xn (+ residual) for up to three weights, and the input half of
 // a SwiGLU block, xn = x or RMSNorm(x).  The reference's counterparts are
 // Linear::forward, RMSNorm::forward and MLP::forward over fp32 weights.
-#include <cmath>
-
-#include "mx4.h"
+#include "mx4_linear.h"
 
 using namespace ember;
 
 namespace {
-
-constexpr int kMaxSeg = 3;  // weights of one ember_mx4_linear call
-
-struct Weight {
-  const uint32_t* codes;
-  const uint32_t* scales;
-};
-
-struct Segs {
-  Weight W[kMaxSeg];
-  const float* res[kMaxSeg];
-  float* y[kMaxSeg];
-  int64_t N[kMaxSeg];
-  int64_t blocks[kMaxSeg + 1];  // prefix sums of column blocks per segment
-  int nseg;
-};
-
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  return g * (1.0f / (1.0f + expf(-g))) * u;
-}
 
 // A workgroup takes 16 rows of x and 64 columns of y: thread (i, j) column j and
 // rows 4 i .. 4 i + 3, the weights' values as they are read, a tile's 64 columns
@@ -38,18 +16,18 @@ constexpr int kRows = 16;
 constexpr int kCols = 64;
 
 template <bool GATE>
-__global__ __launch_bounds__(kThreads) void mx4_linear_kernel(const float* __restrict__ x,
-                                                              int64_t M, int64_t K,
-                                                              const float* __restrict__ norm_w,
-                                                              float eps, Segs sg) {
+__global__ __launch_bounds__(kThreads) void mx4_linear_kernel(Mx4Call sg, Mx4Blocks bl) {
   __shared__ float xs[kRows][64];
   const int j = threadIdx.x % kCols, i = threadIdx.x / kCols;
-  int seg = 0;
-  while (!GATE && seg + 1 < sg.nseg && static_cast<int64_t>(blockIdx.x) >= sg.blocks[seg + 1]) ++seg;
+  const float* x = sg.x;
+  const float* norm_w = sg.norm_w;
+  const int64_t M = sg.M, K = sg.K;
+  int64_t blk = blockIdx.x;
+  const int seg = GATE ? 0 : mx4_segment(bl, sg.nseg, blk);
   const int64_t N = sg.N[seg];
-  const int64_t n = (blockIdx.x - sg.blocks[seg]) * kCols + j;
+  const int64_t n = blk * kCols + j;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kRows;
-  const int64_t kb = (K + 63) / 64, ks = (K + 255) / 256;
+  const int64_t kb = sg.kb, ks = sg.ks;
   const int64_t nb = n / 32, r = n % 32;
   float acc[2][4] = {}, ss[4] = {};
   for (int64_t t = 0; t < kb; ++t) {
@@ -65,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void mx4_linear_kernel(const float* __res
         f32x4 w[2] = {};
         for (int s = 0; s < (GATE ? 2 : 1); ++s) {
           if (n < N) {
-            const Weight& W = sg.W[seg + s];
+            const Mx4Weight& W = sg.W[seg + s];
             const unsigned word = W.codes[(nb * kb + t) * 256 + (32 * h + r) * 4 + q / 2];
             const unsigned sc = W.scales[(nb * ks + t / 4) * 64 + 32 * h + r];
             w[s] = mx4_values(word >> (16 * (q % 2)), sc >> (8 * (t % 4)) & 255u);
@@ -91,10 +69,10 @@ __global__ __launch_bounds__(kThreads) void mx4_linear_kernel(const float* __res
   for (int m = 0; m < 4; ++m) {
     const int64_t row = m0 + 4 * i + m;
     if (row >= M) break;
-    const float sc = norm_w ? 1.0f / sqrtf(ss[m] / static_cast<float>(K) + eps) : 1.0f;
+    const float sc = norm_w ? 1.0f / sqrtf(ss[m] / static_cast<float>(K) + sg.eps) : 1.0f;
     const float v = acc[0][m] * sc;
     float* y = sg.y[seg] + row * N + n;
-    if (GATE) *y = silu_mul(v, acc[1][m] * sc);
+    if (GATE) *y = mx4_silu_mul(v, acc[1][m] * sc);
     else *y = sg.res[seg] ? sg.res[seg][row * N + n] + v : v;
   }
 }
@@ -104,26 +82,38 @@ __global__ __launch_bounds__(kThreads) void mx4_linear_kernel(const float* __res
 bool rows_ok(int64_t M, int64_t K) { return M >= 0 && M <= 0x7fffffff && mx4_sizes_ok(0, K); }
 
 template <bool GATE>
-int launch(const float* x, int64_t M, int64_t K, const float* norm_w, float eps, Segs& sg,
-           ember_stream_t s) {
-  sg.blocks[0] = 0;
-  for (int i = 0; i < sg.nseg; ++i)
-    sg.blocks[i + 1] = sg.blocks[i] + (sg.N[i] + kCols - 1) / kCols;
-  for (int64_t m = 0; m < M; m += int64_t(kRows) * 65535) {
-    Segs part = sg;
-    for (int i = 0; i < sg.nseg; ++i) {
-      part.y[i] += m * sg.N[i];
-      if (part.res[i]) part.res[i] += m * sg.N[i];
+int launch(const Mx4Call& c, hipStream_t st) {
+  Mx4Blocks bl{};
+  for (int i = 0; i < c.nseg; ++i) bl.first[i + 1] = bl.first[i] + (c.N[i] + kCols - 1) / kCols;
+  for (int64_t m = 0; m < c.M; m += int64_t(kRows) * 65535) {
+    Mx4Call part = c;
+    part.x += m * c.K;
+    part.M = c.M - m < int64_t(kRows) * 65535 ? c.M - m : int64_t(kRows) * 65535;
+    for (int i = 0; i < c.nseg; ++i) {
+      part.y[i] += m * c.N[i];
+      if (part.res[i]) part.res[i] += m * c.N[i];
     }
-    const int64_t rows = M - m < int64_t(kRows) * 65535 ? M - m : int64_t(kRows) * 65535;
-    const dim3 grid(static_cast<unsigned>(sg.blocks[GATE ? 1 : sg.nseg]),
-                    static_cast<unsigned>((rows + kRows - 1) / kRows));
-    mx4_linear_kernel<GATE><<<grid, kThreads, 0, as_stream(s)>>>(x + m * K, rows, K, norm_w, eps,
-                                                                 part);
+    const dim3 grid(static_cast<unsigned>(bl.first[GATE ? 1 : c.nseg]),
+                    static_cast<unsigned>((part.M + kRows - 1) / kRows));
+    mx4_linear_kernel<GATE><<<grid, kThreads, 0, st>>>(part, bl);
     const int rc = launch_status();
     if (rc != EMBER_OK) return rc;
   }
   return EMBER_OK;
+}
+
+// The parts of a call that do not depend on its kind.
+Mx4Call call_of(const float* x, int64_t M, int64_t K, const float* norm_w, float eps) {
+  Mx4Call c{};
+  c.x = x;
+  c.norm_w = norm_w;
+  c.eps = eps;
+  c.M = M;
+  c.K = K;
+  c.kb = mx4_col_tiles(K);
+  c.ks = mx4_col_blocks(K);
+  c.x_vec = K % 4 == 0 && aligned16(x) && (!norm_w || aligned16(norm_w));
+  return c;
 }
 
 }  // namespace
@@ -139,23 +129,24 @@ extern "C" int ember_mx4_linear(const float* x, int64_t M, int64_t K, const floa
                                 const float* const* residual, void* workspace,
                                 size_t workspace_bytes, ember_stream_t s) {
   (void)workspace, (void)workspace_bytes;
-  if (!rows_ok(M, K) || nseg < 1 || nseg > kMaxSeg || !codes || !scales || !N || !y)
+  if (!rows_ok(M, K) || nseg < 1 || nseg > kMx4MaxSeg || !codes || !scales || !N || !y)
     return EMBER_EINVAL;
-  Segs sg{};
-  sg.nseg = nseg;
+  Mx4Call c = call_of(x, M, K, norm_w, eps);
+  c.nseg = nseg;
   for (int i = 0; i < nseg; ++i) {
     if (N[i] < 1 || !mx4_sizes_ok(N[i], K)) return EMBER_EINVAL;
     if (M == 0) continue;
     if (!codes[i] || !scales[i] || !y[i]) return EMBER_EINVAL;
     if (!aligned16(codes[i]) || !aligned16(scales[i])) return EMBER_EALIGN;
-    sg.W[i] = {static_cast<const uint32_t*>(codes[i]), static_cast<const uint32_t*>(scales[i])};
-    sg.y[i] = y[i];
-    sg.res[i] = residual ? residual[i] : nullptr;
-    sg.N[i] = N[i];
+    c.W[i] = {static_cast<const uint32_t*>(codes[i]), static_cast<const uint32_t*>(scales[i])};
+    c.y[i] = y[i];
+    c.res[i] = residual ? residual[i] : nullptr;
+    c.N[i] = N[i];
   }
   if (M == 0) return EMBER_OK;
   if (!x) return EMBER_EINVAL;
-  return launch<false>(x, M, K, norm_w, eps, sg, s);
+  if (M <= kMx4FewRows) return mx4_few_rows(c, false, as_stream(s));
+  return launch<false>(c, as_stream(s));
 }
 
 extern "C" int ember_mx4_gateup(const float* x, int64_t M, int64_t K, const float* norm_w,
@@ -168,11 +159,12 @@ extern "C" int ember_mx4_gateup(const float* x, int64_t M, int64_t K, const floa
   if (!x || !gate_codes || !gate_scales || !up_codes || !up_scales || !out) return EMBER_EINVAL;
   for (const void* p : {gate_codes, gate_scales, up_codes, up_scales})
     if (!aligned16(p)) return EMBER_EALIGN;
-  Segs sg{};
-  sg.nseg = 2;
-  sg.W[0] = {static_cast<const uint32_t*>(gate_codes), static_cast<const uint32_t*>(gate_scales)};
-  sg.W[1] = {static_cast<const uint32_t*>(up_codes), static_cast<const uint32_t*>(up_scales)};
-  sg.y[0] = out;
-  sg.N[0] = sg.N[1] = I;
-  return launch<true>(x, M, K, norm_w, eps, sg, s);
+  Mx4Call c = call_of(x, M, K, norm_w, eps);
+  c.nseg = 2;
+  c.W[0] = {static_cast<const uint32_t*>(gate_codes), static_cast<const uint32_t*>(gate_scales)};
+  c.W[1] = {static_cast<const uint32_t*>(up_codes), static_cast<const uint32_t*>(up_scales)};
+  c.y[0] = out;
+  c.N[0] = c.N[1] = I;
+  if (M <= kMx4FewRows) return mx4_few_rows(c, true, as_stream(s));
+  return launch<true>(c, as_stream(s));
 }

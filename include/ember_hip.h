@@ -471,8 +471,10 @@ int ember_mx4_embedding(const int64_t* ids, const void* codes, const void* scale
  * (+ residual[i] [M, N[i]] where residual and residual[i] are not NULL; y[i] may be
  * residual[i]), xn = x where norm_w is NULL, else RMSNorm(x) with weight
  * norm_w [K] and eps.  ember_mx4_gateup: out [M, I] = silu(xn Wg^T) * (xn Wu^T).
- * The codes enter the products as they are held; sums are fp32.  A row of x that
- * is not finite throughout gives a row that is finite nowhere.
+ * The codes enter the products as they are held, xn (before the norm's 1 / rms)
+ * as whole multiples of at most 2^-23 of the largest size in its group of 32 (and of
+ * 2^-127, no less); sums are fp32.  A row of x that is not finite throughout gives
+ * a row that is finite nowhere.
  * `workspace` >= ember_mx4_workspace_bytes(M, K, rows of all the call's weights)
  * (0: none needed; EMBER_EWORKSPACE when smaller), 256-byte aligned (EMBER_EALIGN).
  * Host arrays are read at the call.  Deterministic. */
