@@ -50,5 +50,8 @@ __device__ __forceinline__ float mx4_silu_mul(float g, float u) {
 // Calls of at most kMx4FewRows rows (mx4_few.hip).
 constexpr int kMx4FewRows = 8;
 int mx4_few_rows(const Mx4Call& c, bool gate, hipStream_t st);
+// Calls of more (mx4_many.hip), and the workspace they take.
+size_t mx4_many_rows_bytes(int64_t M, int64_t K);
+int mx4_many_rows(const Mx4Call& c, bool gate, void* workspace, hipStream_t st);
 
 }  // namespace ember
