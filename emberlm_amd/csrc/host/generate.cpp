@@ -83,12 +83,18 @@ Request parse_request(const std::string& text) {
     r.thinking_token_budget = static_cast<int>(integer(*v, "thinking_token_budget"));
   if (const JVal* v = req.find("think_open_ids")) r.think_open_ids = ids(*v, "think_open_ids");
   if (const JVal* v = req.find("think_close_ids")) r.think_close_ids = ids(*v, "think_close_ids");
-  if (const JVal* v = req.find("kv_bits")) {
-    const int64_t bits = integer(*v, "kv_bits");
-    if ((bits != 32 && bits != 4) || v->num != static_cast<double>(bits))  // 4.5 is not 4
-      throw std::runtime_error("request: kv_bits must be 32 or 4");
-    r.kv_bits = static_cast<int>(bits);
-  }
+  const std::pair<const char*, int*> bits_of[] = {{"kv_bits", &r.kv_bits},
+                                                  {"weight_bits", &r.weight_bits},
+                                                  {"embedding_bits", &r.embedding_bits}};
+  for (const auto& [key, to] : bits_of)
+    if (const JVal* v = req.find(key)) {
+      const int64_t bits = integer(*v, key);
+      if ((bits != 32 && bits != 4) || v->num != static_cast<double>(bits))  // 4.5 is not 4
+        throw std::runtime_error(std::string("request: ") + key + " must be 32 or 4");
+      *to = static_cast<int>(bits);
+    }
+  if (r.embedding_bits == 4 && r.weight_bits != 4)
+    throw std::runtime_error("request: embedding_bits 4 needs weight_bits 4");
   return r;
 }
 
@@ -249,12 +255,14 @@ int run(const std::string& model_path, const std::string& request, std::ostream&
     const Request req = parse_request(request);
     const auto t0 = std::chrono::steady_clock::now();
     log << "ctd_generate: weights " << model_path << "\n";
-    const TensorDict weights = load_safetensors(model_path, kHIP0);
+    TensorDict weights = load_safetensors(model_path, kHIP0);
     const nn::LlamaConfig cfg = model_config.empty() ? nn::autodetect_config(weights)
                                                      : train::load_model_config(model_config);
     log << "ctd_generate: " << cfg.num_hidden_layers << " layers of width " << cfg.hidden_size
         << ", vocabulary " << cfg.vocab_size << "\n";
-    const nn::Model model = nn::build_model(weights, cfg);
+    nn::Model model = nn::build_model(weights, cfg);
+    weights.clear();
+    if (req.weight_bits == 4) model.quantize_weights(req.embedding_bits == 4);
     log << "ctd_generate: loaded in " << seconds_since(t0) << " s\n";
 
     const int prompt_len = static_cast<int>(req.input_ids.size());

@@ -125,9 +125,11 @@ Tensor hidden_states(const Model& m, const Tensor& input_ids, KVCache* cache,
 
 Tensor Model::forward(const Tensor& input_ids, KVCache* cache, int position_start) const {
   autograd::NoGradGuard ng;
-  Tensor h = norm.forward(hidden_states(*this, input_ids, cache, position_start));
+  Tensor h = hidden_states(*this, input_ids, cache, position_start);
+  if (embed_tokens.mx4.defined())
+    return ops::linear_mx4(h, norm.weight, norm.eps, {&embed_tokens.mx4})[0];
   Linear lm_head{embed_tokens.weight};  // tied head
-  return lm_head.forward(h);
+  return lm_head.forward(norm.forward(h));
 }
 
 Tensor Model::forward_last_logits(const Tensor& input_ids, KVCache* cache,
@@ -145,6 +147,8 @@ Tensor Model::forward_last_logits(const Tensor& input_ids, KVCache* cache,
                                    static_cast<const float*>(h.data_ptr()) + (b * T + T - 1) * H,
                                    H * sizeof(float), 2, runtime::compute_stream()));
   }
+  if (embed_tokens.mx4.defined())
+    return ops::linear_mx4(last, norm.weight, norm.eps, {&embed_tokens.mx4})[0];
   if (B <= ops::kDecodeMaxRows)  // final RMSNorm folded into the LM-head GEMV
     return ops::decode_linear(last, norm.weight, norm.eps, {embed_tokens.weight})[0];
   Linear lm_head{embed_tokens.weight};
@@ -160,6 +164,10 @@ Tensor train_hidden(const Model& m, const Tensor& input_ids) {
   Tensor h = m.embed_tokens.forward(input_ids);
   for (size_t i = 0; i < m.layers.size(); ++i) {
     const TransformerBlock& layer = m.layers[i];
+    if (layer.mx4()) {
+      h = layer.forward(h);
+      continue;
+    }
     if (m.gradient_checkpointing) {
       // checkpoint() runs fn under no-grad in the forward pass and with grad
       // enabled when the backward pass re-runs it; the re-run only
@@ -192,9 +200,19 @@ Tensor train_hidden(const Model& m, const Tensor& input_ids) {
 }  // namespace
 
 Tensor Model::forward_train_logits(const Tensor& input_ids) const {
-  Linear lm_head{embed_tokens.weight};  // tied head
+  Linear lm_head{embed_tokens.weight, embed_tokens.mx4};  // tied head
   return lm_head.forward(train_hidden(*this, input_ids));
 }
+
+namespace {
+
+// The tied LM head's fp32 table; one in 4 bits is read back for the call.
+Tensor head_table(const Model& m) {
+  return m.embed_tokens.mx4.defined() ? ops::dequantize_mx4(m.embed_tokens.mx4)
+                                      : m.embed_tokens.weight;
+}
+
+}  // namespace
 
 // The losses run the tied LM head and the cross-entropy together a chunk of
 // rows at a time (ops::linear_cross_entropy_masked): the same loss as
@@ -206,7 +224,7 @@ Tensor Model::forward_train(const Tensor& input_ids, const Tensor& targets) cons
   CTD_CHECK(ember_fill(static_cast<float*>(ones.data_ptr()), total, 1.0f,
                        runtime::compute_stream()));
   return ops::linear_cross_entropy_masked(h.reshape({total, h.shape().back()}),
-                                          embed_tokens.weight, targets.reshape({total}), ones);
+                                          head_table(*this), targets.reshape({total}), ones);
 }
 
 Tensor Model::forward_train_masked(const Tensor& input_ids, const Tensor& targets,
@@ -214,7 +232,7 @@ Tensor Model::forward_train_masked(const Tensor& input_ids, const Tensor& target
   const int64_t total = input_ids.numel();
   Tensor h = train_hidden(*this, input_ids);
   return ops::linear_cross_entropy_masked(h.reshape({total, h.shape().back()}),
-                                          embed_tokens.weight, targets.reshape({total}),
+                                          head_table(*this), targets.reshape({total}),
                                           loss_mask.reshape({total}));
 }
 
@@ -302,7 +320,32 @@ Model build_model(const TensorDict& w, const LlamaConfig& cfg) {
   return m;
 }
 
+void Model::quantize_weights(bool table) {
+  autograd::NoGradGuard ng;
+  auto hold = [](Tensor& w, ops::Mx4Weight& mx4) {
+    if (mx4.defined()) return;
+    mx4 = ops::quantize_mx4(w);
+    w = Tensor{};
+  };
+  for (TransformerBlock& b : layers)
+    for (Linear* l : {&b.self_attn.q_proj, &b.self_attn.k_proj, &b.self_attn.v_proj,
+                      &b.self_attn.o_proj, &b.mlp.gate_proj, &b.mlp.up_proj, &b.mlp.down_proj})
+      hold(l->weight, l->mx4);
+  if (table) hold(embed_tokens.weight, embed_tokens.mx4);
+  auto settle = [](Tensor& t) {
+    if (t.defined()) t.requires_grad_(false);
+  };
+  settle(embed_tokens.weight);
+  settle(norm.weight);
+  for (TransformerBlock& b : layers)
+    for (RMSNorm* n : {&b.input_layernorm, &b.post_attention_layernorm, &b.self_attn.q_norm,
+                       &b.self_attn.k_norm})
+      settle(n->weight);
+}
+
 Model::NamedParameters Model::collect_parameters() {
+  if (weights_quantized() || embed_tokens.mx4.defined())
+    throw std::runtime_error("collect_parameters: weights held in 4 bits are no parameters");
   NamedParameters out;
   auto take = [&out](std::string name, Tensor& t, bool decay) {
     t.requires_grad_(true);

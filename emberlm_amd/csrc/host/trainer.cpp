@@ -132,6 +132,12 @@ Tensor& param_at(Trainer* tr, int64_t i) {
   return tr->named.all[static_cast<size_t>(i)].second;
 }
 
+// For calls that make no sense without parameters.
+void require_parameters(const Trainer* tr, const char* call) {
+  if (tr->named.all.empty())
+    throw std::runtime_error(std::string(call) + ": the weights are held in 4 bits");
+}
+
 void check_numel(const Tensor& t, int64_t numel) {
   if (t.numel() != numel) throw std::runtime_error("numel mismatch");
 }
@@ -285,6 +291,21 @@ int ctd_trainer_set_checkpoint_bits(ctd_trainer_t t, int32_t bits) {
   });
 }
 
+int ctd_trainer_quantize_weights(ctd_trainer_t t, int32_t table) {
+  return guarded([&] {
+    Trainer* tr = as_trainer(t);
+    if (tr->opt) tr->opt->wait_idle();
+    runtime::synchronize();
+    tr->model.recompute_hook = nullptr;
+    tr->opt.reset();
+    tr->named = {};
+    tr->decay.clear();
+    tr->opt_index.clear();
+    tr->model.quantize_weights(table != 0);
+    runtime::synchronize();
+  });
+}
+
 int ctd_trainer_set_checkpointing(ctd_trainer_t t, int32_t on) {
   return guarded([&] { as_trainer(t)->model.gradient_checkpointing = on != 0; });
 }
@@ -364,6 +385,7 @@ int ctd_trainer_block_step(ctd_trainer_t t, int64_t layer, const float* x, const
     Trainer* tr = as_trainer(t);
     if (layer < 0 || layer >= static_cast<int64_t>(tr->model.layers.size()))
       throw std::runtime_error("layer index out of range");
+    require_parameters(tr, "block_step");
     const auto& blk = tr->model.layers[static_cast<size_t>(layer)];
     const int64_t d = tr->model.config.hidden_size;
     Tensor xin = Tensor::from_host(x, {B, T, d}, DType::kFloat32, kHIP0);
@@ -398,6 +420,7 @@ int ctd_trainer_make_optimizer(ctd_trainer_t t, float lr, float weight_decay, fl
                                float beta2, float eps, int32_t offload, int64_t chunk_elems) {
   return guarded([&] {
     Trainer* tr = as_trainer(t);
+    require_parameters(tr, "make_optimizer");
     // Two groups like ctd_train (main.cpp:299-311): decay, then no_decay with wd 0.
     std::vector<optim::ParamGroup> groups{{tr->named.decay, lr, weight_decay},
                                           {tr->named.no_decay, lr, 0.0f}};
@@ -654,6 +677,7 @@ int ctd_trainer_save(ctd_trainer_t t, const char* path) {
   return guarded([&] {
     Trainer* tr = as_trainer(t);
     runtime::synchronize();
+    require_parameters(tr, "save");
     save_safetensors(tr->named.all, path);
     if (tr->opt) train::save_optimizer_state(*tr->opt, tr->named, train::opt_path_for(path));
   });
@@ -663,6 +687,7 @@ int ctd_trainer_load(ctd_trainer_t t, const char* path) {
   return guarded([&] {
     Trainer* tr = as_trainer(t);
     const SafetensorsReader file(path);  // each parameter is read straight into place
+    require_parameters(tr, "load");
     for (auto& [name, p] : tr->named.all) {
       if (!file.find(name)) throw std::runtime_error(std::string("load: ") + path + " lacks " + name);
       file.read(name, p);

@@ -120,6 +120,7 @@ _SIGS = {
     "ctd_trainer_generate": (i32, [vp, lptr, i64, i32, f32, i32, f32, u64, i64, lptr,
                                    C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     "ctd_trainer_set_checkpoint_bits": (i32, [vp, i32]),
+    "ctd_trainer_quantize_weights": (i32, [vp, i32]),
     "ctd_kvcache_create_bits": (i32, [vp, i64, i64, i32, C.POINTER(vp)]),
     "ctd_trainer_generate_bits": (i32, [vp, lptr, i64, i32, f32, i32, f32, u64, i64, i32, lptr,
                                         C.POINTER(C.c_double), C.POINTER(C.c_double)]),
@@ -267,6 +268,13 @@ class Trainer:
     def set_checkpoint_bits(self, bits):
         """How a checkpointed block's input is held: 32 bits (as it is) or 8."""
         _ck(lib().ctd_trainer_set_checkpoint_bits(self.h, bits), "set_checkpoint_bits")
+
+    def quantize_weights(self, table=False):
+        """Holds the projections (and, with table, the embedding table and LM head) in 4 bits
+        from here on: forward, generate and losses run on them; there are no parameters,
+        gradients or optimizer any more."""
+        _ck(lib().ctd_trainer_quantize_weights(self.h, int(bool(table))), "quantize_weights")
+        self.names, self.numels, self.decay = [], [], []
 
     def set_checkpointing(self, on):
         _ck(lib().ctd_trainer_set_checkpointing(self.h, int(on)), "set_checkpointing")

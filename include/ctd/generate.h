@@ -8,7 +8,10 @@
 //    "temperature": 1.0, "top_k": 0, "top_p": 0.0, "seed": 0,
 //    "eos_ids": [int...],
 //    "thinking_token_budget": 0, "think_open_ids": [...], "think_close_ids": [...],
-//    "kv_bits": 32}                     32 or 4 (added in this build)
+//    "kv_bits": 32,                     32 or 4 (added in this build)
+//    "weight_bits": 32,                 32 or 4: the blocks' projections (added)
+//    "embedding_bits": 32}              32 or 4: the embedding table and LM head (added;
+//                                       4 only beside weight_bits 4)
 // Reply: one JSON line per generated token {"token":id}, then
 //   {"done":true,"generated_tokens":n,"reason":"max_tokens"|"eos"|"max_seq_len"},
 // or {"done":true,"reason":"empty_prompt"|"max_seq_len"} before any token, or
@@ -35,6 +38,10 @@ struct Request {
   std::vector<int64_t> think_open_ids;
   std::vector<int64_t> think_close_ids;
   int kv_bits = 32;  // 4: a KV cache held in 4 bits (nn::KVCache::allocate)
+  // 4: run() holds the model's weights in 4 bits (nn::Model::quantize_weights);
+  // generate_loop takes the model as it is.
+  int weight_bits = 32;
+  int embedding_bits = 32;
 };
 
 // Parses a request; throws std::runtime_error on bad JSON or field types.

@@ -78,9 +78,17 @@ struct Attention {
     const int64_t B = x.shape()[0];
     const int64_t T = x.shape()[1];
     const int H = num_heads, Hk = num_kv_heads, D = head_dim;
-    Tensor Q = q_proj.forward(x).reshape({B, T, H, D});
-    Tensor K = k_proj.forward(x).reshape({B, T, Hk, D});
-    Tensor V = v_proj.forward(x).reshape({B, T, Hk, D});
+    return context_of(q_proj.forward(x).reshape({B, T, H, D}),
+                      k_proj.forward(x).reshape({B, T, Hk, D}),
+                      v_proj.forward(x).reshape({B, T, Hk, D}), kv, position_start);
+  }
+
+  // The same from the projections: Q [B,T,H,D], K and V [B,T,Hk,D], Q and K
+  // before their norms and rotation (without norms they are rotated in place).
+  Tensor context_of(Tensor Q, Tensor K, const Tensor& V, KVLayer* kv, int position_start) const {
+    autograd::NoGradGuard ng;
+    const int64_t B = Q.shape()[0], T = Q.shape()[1];
+    const int H = num_heads, D = head_dim;
     if (has_qk_norm()) {
       Q = ops::qk_norm_rope(Q, q_norm.weight, q_norm.eps, position_start, rope_theta,
                             rope_scaling);

@@ -80,6 +80,15 @@ struct Model {
   Tensor forward_train_masked(const Tensor& input_ids, const Tensor& targets,
                               const Tensor& loss_mask) const;
 
+  // Brings the projections of every block into 4 bits (ops/quant.h; and, with
+  // table, the embedding table, which is the LM head too) and lets go of their fp32
+  // values.  forward, forward_last_logits and generation then run on the 4-bit
+  // weights; the training forwards give logits and losses without a graph (no
+  // tensor of the model requires grad any more), and collect_parameters throws.  A
+  // second call may add the table.
+  void quantize_weights(bool table = false);
+  bool weights_quantized() const { return !layers.empty() && layers[0].mx4(); }
+
   struct NamedParameters {
     std::vector<std::pair<std::string, Tensor>> all;
     std::vector<Tensor> decay;

@@ -88,6 +88,11 @@ int ctd_trainer_set_checkpointing(ctd_trainer_t t, int32_t on);
  * default: as it is) or 8 (Model::checkpoint_bits).  Also holds for
  * ctd_trainer_block_step's checkpoint. */
 int ctd_trainer_set_checkpoint_bits(ctd_trainer_t t, int32_t bits);
+/* Holds the model's projections (and, with table != 0, its embedding table and
+ * LM head) in 4 bits from here on (Model::quantize_weights): forward, generation
+ * and losses run on them.  The handle has no parameters, gradients or optimizer
+ * any more: the calls that need them fail. */
+int ctd_trainer_quantize_weights(ctd_trainer_t t, int32_t table);
 /* Batch: ids/targets int64 [B,T], mask fp32 [B,T] (NULL = all ones), host memory. */
 int ctd_trainer_set_batch(ctd_trainer_t t, const int64_t* ids, const int64_t* targets,
                           const float* mask, int64_t B, int64_t T);

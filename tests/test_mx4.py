@@ -1,10 +1,14 @@
 """CPU checks of the 4-bit weights: the rule in 64 bits and the refusals of the entry points."""
 import ctypes as C
+import json
+import os
+import subprocess
 
 import numpy as np
 import pytest
 
 from emberlm_amd import capi
+from emberlm_amd import trainer as TR
 from oracle import mx4 as OM
 
 P = C.c_void_p(4096)  # never dereferenced
@@ -134,3 +138,26 @@ def test_workspace_is_asked_for(M):
         assert _gateup(M=M, K=2048, N=32, need=need - 1) == -2
         assert _gateup(M=M, K=2048, N=32, ws=None) == -2
         assert _gateup(M=M, K=2048, N=32, ws=ODD) == -3
+
+
+def _generate(request):
+    exe = os.path.join(os.path.dirname(TR.LIB_PATH), "ctd_generate")
+    r = subprocess.run([exe, "--model", "/nonexistent.safetensors"],
+                       input='{"input_ids": [1], %s}' % request, capture_output=True, text=True,
+                       timeout=60)
+    assert r.returncode == 1
+    return json.loads(r.stdout)["error"]
+
+
+@pytest.mark.parametrize("bits", ["4.5", "32.25", str(2 ** 32 + 4), "-4", "0", "8", "16"])
+@pytest.mark.parametrize("key", ["weight_bits", "embedding_bits"])
+def test_bits_of_a_request_are_32_or_4(key, bits):
+    assert key + " must be 32 or 4" in _generate('"%s": %s' % (key, bits))
+
+
+def test_bits_of_a_request_that_are_taken():
+    """The request passes; what fails then is the model file."""
+    for request in ('"weight_bits": 4', '"weight_bits": 32, "embedding_bits": 32',
+                    '"weight_bits": 4.0, "embedding_bits": 4', '"weight_bits": 4, "kv_bits": 4'):
+        assert "bits" not in _generate(request)
+    assert "needs weight_bits 4" in _generate('"embedding_bits": 4')
