@@ -26,7 +26,7 @@ Mx4Call call_of(const float* x, int64_t M, int64_t K, const float* norm_w, float
 }
 
 int run(const Mx4Call& c, bool gate, void* workspace, size_t workspace_bytes, hipStream_t st) {
-  if (c.M <= kMx4FewRows) return mx4_few_rows(c, gate, st);
+  if (mx4_few(c.M, c.K)) return mx4_few_rows(c, gate, st);
   if (!workspace || workspace_bytes < mx4_many_rows_bytes(c.M, c.K)) return EMBER_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return EMBER_EALIGN;
   return mx4_many_rows(c, gate, workspace, st);
@@ -35,7 +35,7 @@ int run(const Mx4Call& c, bool gate, void* workspace, size_t workspace_bytes, hi
 }  // namespace
 
 extern "C" size_t ember_mx4_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-  if (!rows_ok(M, K) || N < 0 || M <= kMx4FewRows) return 0;
+  if (!rows_ok(M, K) || N < 0 || mx4_few(M, K)) return 0;
   return mx4_many_rows_bytes(M, K);
 }
 
