@@ -60,9 +60,13 @@ __device__ __forceinline__ unsigned over_8(unsigned v, F f) {
   return f(v, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true)));
 }
 
+// Four columns of a row; zeros past its end.  once: past the caches.
 __device__ __forceinline__ f32x4 load_x(const float* __restrict__ row, int64_t c, int64_t K,
-                                        bool vec) {
-  if (vec) return c < K ? *reinterpret_cast<const f32x4*>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+                                        bool vec, bool once) {
+  if (vec) {
+    const f32x4* at = reinterpret_cast<const f32x4*>(row + c);
+    return c >= K ? f32x4{0.f, 0.f, 0.f, 0.f} : once ? __builtin_nontemporal_load(at) : *at;
+  }
   f32x4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = c + e < K ? row[c + e] : 0.f;
@@ -76,7 +80,7 @@ __device__ __forceinline__ f32x4 load_x(const float* __restrict__ row, int64_t c
 // beginning of its neighbour's.  Rows past M are left as they are (what is
 // multiplied with them is not stored).
 __global__ __launch_bounds__(kSplitThreads) void mx4_split_kernel(Mx4Call c, Space sp,
-                                                                  int64_t blocks) {
+                                                                  int64_t blocks, bool once) {
   __shared__ float sums[8][4];
   const int q = threadIdx.x / kWave, r = threadIdx.x % kWave / 8, c8 = threadIdx.x % 8, j = c8 % 4;
   const int word = 3 * (c8 / 4) + j;  // of a lane's six
@@ -86,13 +90,13 @@ __global__ __launch_bounds__(kSplitThreads) void mx4_split_kernel(Mx4Call c, Spa
     f32x4 v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      v[h] = load_x(c.x + row * c.K, kb * 64 + 32 * h + 4 * c8, c.K, c.x_vec);
+      v[h] = load_x(c.x + row * c.K, kb * 64 + 32 * h + 4 * c8, c.K, c.x_vec, once);
     if (c.norm_w) {
       float ss = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         ss += v[h].x * v[h].x + v[h].y * v[h].y + v[h].z * v[h].z + v[h].w * v[h].w;
-        v[h] *= load_x(c.norm_w, kb * 64 + 32 * h + 4 * c8, c.K, c.x_vec);
+        v[h] *= load_x(c.norm_w, kb * 64 + 32 * h + 4 * c8, c.K, c.x_vec, false);
       }
       ss = __uint_as_float(over_8(__float_as_uint(ss), [](unsigned a, unsigned b) {
         return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
@@ -540,6 +544,12 @@ Kernel kernel_of(const Mx4Call& c, bool gate) {
   return t_mid <= t_large ? Kernel::kMid : Kernel::kLarge;
 }
 
+// An x of more values than these is read past the caches, which its digits then have to
+// themselves until the product reads them (4096 x 6144, 100 MB: 195 -> 178 us in all); a
+// smaller one may still be there when the product's residual or the caller wants it (2048 x
+// 6144: 102 us, read past them 105).
+constexpr int64_t kKeep = int64_t(1) << 24;
+
 // Rows whose digits take a quarter of a GB, whole blocks of 256: a longer x is taken
 // in pieces of that many.
 int64_t piece_rows(int64_t M, int64_t kb) {
@@ -572,7 +582,7 @@ int ember::mx4_many_rows(const Mx4Call& call, bool gate, void* workspace, hipStr
     }
     const int64_t blocks = (c.M + 7) / 8 * c.ks;
     mx4_split_kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)), kSplitThreads, 0,
-                       st>>>(c, sp, blocks);
+                       st>>>(c, sp, blocks, c.M * c.K > kKeep);
     int rc = launch_status();
     if (rc != EMBER_OK) return rc;
     switch (kernel_of(c, gate)) {
