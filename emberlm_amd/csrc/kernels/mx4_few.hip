@@ -405,8 +405,14 @@ int by_waves(const Mx4Call& c, hipStream_t st) {
 int ember::mx4_few_rows(const Mx4Call& c, bool gate, hipStream_t st) {
   int64_t tiles = 0;
   for (int i = 0; i < (gate ? 1 : c.nseg); ++i) tiles += (c.N[i] + 15) / 16;
+  // Workgroups of one tile of columns as long as the GPU holds them all at once (two a CU
+  // up to six rows, by registers and LDS), else of more: a workgroup cuts x for itself (8
+  // rows of K = 2048 to 2 x 6144 columns: 16.9 us with 384 workgroups, 10.7 with 192).
   const int64_t slots = c.M <= 2 * kTokens ? 512 : 256;
   if (gate) return tiles <= slots ? by_waves<2, true>(c, st) : by_waves<4, true>(c, st);
+  // Twice the waves for a long K where a CU has one workgroup at most (one row of K = 8192,
+  // N = 2048 7.4 -> 6.7 us; with N = 8192 11.1, and 12.8 so).
+  if (tiles <= 256 && c.ks >= 16 && c.M <= kTokens) return launch<1, 1, 16, false>(c, st);
   if (tiles <= slots) return by_waves<1, false>(c, st);
   return tiles <= 2 * slots ? by_waves<2, false>(c, st) : by_waves<4, false>(c, st);
 }
