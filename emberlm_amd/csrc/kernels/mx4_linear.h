@@ -48,11 +48,13 @@ __device__ __forceinline__ float mx4_silu_mul(float g, float u) {
 }
 
 // Calls of few rows (mx4_few.hip).  Each of its workgroups cuts all of x into digits
-// for itself, which for seven rows and more of a long K takes longer than a launch
-// that does it once: 8 rows of K = 8192, N = 2048 22.5 us there, 18.3 in mx4_many.hip;
-// of K = 2048 7.6 and 8.5.
+// for itself, which for an x of many values takes longer than a launch that does it
+// once.  With N = 2048, there and in mx4_many.hip: 8 rows of K = 8192 22.5 us and 11.4,
+// 8 of 4096 11.4 and 10.7, 4 of 6144 9.7 and 11, 8 of 2048 7.6 and 8.5.
 constexpr int kMx4FewRows = 8;
-inline bool mx4_few(int64_t M, int64_t K) { return M <= 6 || (M <= kMx4FewRows && K <= 3200); }
+inline bool mx4_few(int64_t M, int64_t K) {
+  return M <= 3 || (M <= kMx4FewRows && M * K <= 30000);
+}
 int mx4_few_rows(const Mx4Call& c, bool gate, hipStream_t st);
 // Calls of more (mx4_many.hip), and the workspace they take.
 size_t mx4_many_rows_bytes(int64_t M, int64_t K);

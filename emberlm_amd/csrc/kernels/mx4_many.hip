@@ -44,12 +44,14 @@ struct Space {
   uint8_t* digits;   // [R / 64][kb][2][kDigits][kDigitBytes]: 15 KB for 64 rows by 64 columns
   uint8_t* scales;   // [R / 32][ks][64][4]
   float* squares;    // [R][ks]
+  float* parts;      // [kMostParts][2][16][64]: sums of splits of K (the small kernel's)
 };
+constexpr int kMostParts = 256;  // workgroups of a launch that splits K
 constexpr size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t digit_bytes(int64_t tiles, int64_t kb) { return static_cast<size_t>(tiles * kb) * kTileBytes; }
 size_t space_bytes(int64_t tiles, int64_t kb, int64_t ks) {
   return round256(digit_bytes(tiles, kb)) + round256(static_cast<size_t>(tiles * ks) * 256) +
-         round256(static_cast<size_t>(tiles * 32 * ks) * 4);
+         round256(static_cast<size_t>(tiles * 32 * ks) * 4) + kMostParts * 8192;
 }
 
 // v of eight neighbouring lanes combined, in each of them: lane ^ 1, ^ 2, ^ 7.
@@ -387,21 +389,26 @@ __global__ __launch_bounds__(S::kThreads) void mx4_gemm_kernel(Mx4Call c, Space 
 
 // Few tiles: a workgroup takes 32 rows by 32 columns (GATE: of the gate's and the
 // up projection's both), its eight waves an eighth of K each, operands straight
-// from memory to registers; the waves' sums are joined over LDS.  What counts here
-// is the time from the first load to the last sum, not the bytes.
+// from memory to registers; the waves' sums are joined over LDS.  What bounds it is a
+// CU's path to its L2 (8.7 KB a tile of K, 64 bytes a cycle), so where the tiles are few
+// and K is long, several workgroups take a tile, each a part of K, and leave their sums
+// in the workspace, which mx4_join_kernel adds up in their order and stores.  (8 rows of K =
+// 8192, N = 2048 18.1 -> 11.4 us; joined by the last workgroup to arrive, 13.2.)
 constexpr int kSmallWaves = 8;
 
 template <bool GATE>
 __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c, Space sp,
                                                                        Mx4Blocks bl,
-                                                                       unsigned col_blocks) {
+                                                                       unsigned col_blocks,
+                                                                       int splits) {
   constexpr int TN = GATE ? 2 : 1;
   __shared__ float red[kSmallWaves][TN][16][kWave];
   __shared__ float factor[32];
   const int lane = threadIdx.x & (kWave - 1);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t mb = blockIdx.x / col_blocks;
-  int64_t nblk = blockIdx.x % col_blocks;
+  const unsigned tile = blockIdx.x / splits, split = blockIdx.x % splits;
+  const int64_t mb = tile / col_blocks;
+  int64_t nblk = tile % col_blocks;
   const int seg = GATE ? 0 : mx4_segment(bl, c.nseg, nblk);
   const int kb = static_cast<int>(c.kb);
   const uint8_t* a_at = sp.digits + (mb / 2 * kb * 2 + mb % 2) * int64_t(kTileBytes) + lane * 16;
@@ -434,10 +441,11 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c
   };
   f32x16 hi[TN] = {}, lo[TN] = {};
   Operands next;
-  if (w < kb) load(next, w);
-  for (int k = w; k < kb; k += kSmallWaves) {
+  const int step = kSmallWaves * splits, first = kSmallWaves * split + w;
+  if (first < kb) load(next, first);
+  for (int k = first; k < kb; k += step) {
     const Operands o = next;
-    if (k + kSmallWaves < kb) load(next, k + kSmallWaves);
+    if (k + step < kb) load(next, k + step);
     const int shift = k % 4 * 8;
 #pragma unroll
     for (int p = kDigits - 1; p >= 0; --p) {
@@ -465,6 +473,24 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c
   }
   __syncthreads();
   // Two of the 16 accumulator registers a wave; the waves' parts in their order.
+  float sum[2][TN];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      sum[j][t] = 0.f;
+#pragma unroll
+      for (int u = 0; u < kSmallWaves; ++u) sum[j][t] += red[u][t][2 * w + j][lane];
+    }
+  if (splits > 1) {
+    // [tile][split][t][16][64]
+    float* parts = sp.parts + static_cast<size_t>(blockIdx.x) * (TN * 1024) + lane;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int t = 0; t < TN; ++t) parts[(t * 16 + 2 * w + j) * 64] = sum[j][t];
+    return;
+  }
   const int64_t N = c.N[seg], n = nblk * 32 + lane % 32;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -473,16 +499,48 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c
     if (m >= c.M || n >= N) continue;
     float v[TN];
 #pragma unroll
-    for (int t = 0; t < TN; ++t) {
-      v[t] = 0.f;
-#pragma unroll
-      for (int u = 0; u < kSmallWaves; ++u) v[t] += red[u][t][i][lane];
-      if (c.norm_w) v[t] *= factor[r];
-    }
+    for (int t = 0; t < TN; ++t) v[t] = c.norm_w ? sum[j][t] * factor[r] : sum[j][t];
     float* y = c.y[seg] + m * N + n;
     if constexpr (GATE) *y = mx4_silu_mul(v[0], v[1]);
     else *y = c.res[seg] ? c.res[seg][m * N + n] + v[0] : v[0];
   }
+}
+
+// The sums of a tile's splits, a quarter of the tile a workgroup.
+template <bool GATE>
+__global__ __launch_bounds__(256) void mx4_join_kernel(Mx4Call c, Space sp, Mx4Blocks bl,
+                                                       unsigned col_blocks, int splits) {
+  constexpr int TN = GATE ? 2 : 1;
+  const int lane = threadIdx.x % kWave, i = blockIdx.x % 4 * 4 + threadIdx.x / kWave;
+  const unsigned tile = blockIdx.x / 4;
+  const int64_t mb = tile / col_blocks;
+  int64_t nblk = tile % col_blocks;
+  const int seg = GATE ? 0 : mx4_segment(bl, c.nseg, nblk);
+  const int64_t N = c.N[seg], n = nblk * 32 + lane % 32;
+  const int64_t m = mb * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+  if (m >= c.M || n >= N) return;
+  float v[TN] = {};
+  for (int u = 0; u < splits; ++u)
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+      v[t] += sp.parts[((static_cast<size_t>(tile) * splits + u) * TN + t) * 1024 + i * 64 + lane];
+  if (c.norm_w) {
+    float sum = 0.f;
+    for (int64_t k = 0; k < c.ks; ++k) sum += sp.squares[m * c.ks + k];
+    const float rstd = 1.0f / sqrtf(sum / static_cast<float>(c.K) + c.eps);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) v[t] *= rstd;
+  }
+  float* y = c.y[seg] + m * N + n;
+  if constexpr (GATE) *y = mx4_silu_mul(v[0], v[1]);
+  else *y = c.res[seg] ? c.res[seg][m * N + n] + v[0] : v[0];
+}
+
+// How many workgroups of the small kernel share a tile: as many as the GPU has CUs for, four
+// at most, and four tiles of K a wave at least (at K = 2048 two took 10.7 us for one's 9.9).
+int64_t small_splits(int64_t tiles, int64_t kb) {
+  const int64_t splits = std::min<int64_t>(kMostParts / std::max<int64_t>(tiles, 1), kb / 32);
+  return std::max<int64_t>(std::min<int64_t>(splits, 4), 1);
 }
 
 template <bool GATE>
@@ -490,9 +548,15 @@ int launch_small(const Mx4Call& c, const Space& sp, hipStream_t st) {
   Mx4Blocks bl{};
   for (int i = 0; i < c.nseg; ++i) bl.first[i + 1] = bl.first[i] + mx4_row_tiles(c.N[i]);
   const int64_t cols = bl.first[GATE ? 1 : c.nseg], rows = mx4_row_tiles(c.M);
-  if (cols * rows > 0x7fffffff) return EMBER_EINVAL;
-  mx4_small_kernel<GATE><<<static_cast<unsigned>(cols * rows), kSmallWaves * kWave, 0, st>>>(
-      c, sp, bl, static_cast<unsigned>(cols));
+  const int64_t splits = small_splits(cols * rows, c.kb);
+  if (cols * rows * splits > 0x7fffffff) return EMBER_EINVAL;
+  mx4_small_kernel<GATE><<<static_cast<unsigned>(cols * rows * splits), kSmallWaves * kWave, 0,
+                           st>>>(c, sp, bl, static_cast<unsigned>(cols),
+                                 static_cast<int>(splits));
+  const int rc = launch_status();
+  if (rc != EMBER_OK || splits == 1) return rc;
+  mx4_join_kernel<GATE><<<static_cast<unsigned>(4 * cols * rows), 256, 0, st>>>(
+      c, sp, bl, static_cast<unsigned>(cols), static_cast<int>(splits));
   return launch_status();
 }
 
@@ -518,7 +582,7 @@ int launch_gemm(const Mx4Call& c, const Space& sp, hipStream_t st) {
 //   tiles of 64 x 128 take 0.38 a CU, so 1.3 times as long a value, in smaller
 //   rounds;
 //   the small kernel's 32 x 32 take 0.105, 2.5 times as long a value, but an eighth
-//   of K's latency.
+//   of K's latency, or less where several workgroups share a tile.
 // Linear K = 2048, N = 4096 in the order small, 64 x 128, 128 x 256: 128 rows 13.8,
 // 17.4, 33.7 us; 512 rows 35.1, 26.6, 37.3; 2048 rows 118, 65.9, 57.2.
 enum class Kernel { kSmall, kMid, kLarge };
@@ -536,8 +600,9 @@ Kernel kernel_of(const Mx4Call& c, bool gate) {
   large *= (c.M + 127) / 128;
   const double kb = static_cast<double>(c.kb);
   const double rounds = std::floor(large / 256), rest = large / 256 - rounds;
-  const double t_small = 1 + 2.5 * std::ceil(small / 768) +
-                         0.105 * twice * kb * std::max(small / 256, 1.0);
+  const double splits = static_cast<double>(small_splits(static_cast<int64_t>(small), c.kb));
+  const double t_small = 1 + 2.5 * std::ceil(small / 768) + (splits > 1 ? 2.5 : 0) +
+                         0.105 * twice * kb * std::max(small / 256, 1.0 / splits);
   const double t_mid = 5 + 0.38 * kb * std::ceil(mid / 256);
   const double t_large = rounds * (6 + 1.17 * kb) + (rest > 0 ? 6 + (0.72 + 0.45 * rest) * kb : 0);
   if (t_small <= t_mid && t_small <= t_large) return Kernel::kSmall;
@@ -572,6 +637,8 @@ int ember::mx4_many_rows(const Mx4Call& call, bool gate, void* workspace, hipStr
   sp.scales = p;
   p += round256(static_cast<size_t>(tiles * call.ks) * 256);
   sp.squares = reinterpret_cast<float*>(p);
+  p += round256(static_cast<size_t>(tiles * 32 * call.ks) * 4);
+  sp.parts = reinterpret_cast<float*>(p);
   for (int64_t m = 0; m < call.M; m += rows) {
     Mx4Call c = call;
     c.M = std::min(rows, call.M - m);
