@@ -140,7 +140,7 @@ __device__ __forceinline__ void cut_x(const Mx4Call& c, int64_t kblk, uint8_t* m
     // the digits' factors 2^-5 .. 2^-20
     const int byte = top >= 0x7f800000u ? 255 : max(static_cast<int>(top >> 23) - 3, 20);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] = __builtin_ldexpf(t[e], 127 - byte);
+    for (int e = 0; e < 4; ++e) t[e] = byte == 255 ? 0.f : __builtin_ldexpf(t[e], 127 - byte);
     uint8_t* row = mine + (m / kTokens) * kTileLds + (m % kTokens) * kDigits * kRowBytes;
 #pragma unroll
     for (int p = 0; p < kDigits; ++p) {
@@ -383,6 +383,7 @@ int launch(const Mx4Call& c, hipStream_t st) {
       return launch_status();
     }
   }
+  if (!mx4_launch_ok(total, W * kWave)) return EMBER_EINVAL;
   mx4_few_kernel<TT, NT, W, GATE><<<static_cast<unsigned>(total), W * kWave, 0, st>>>(c, bl);
   return launch_status();
 }

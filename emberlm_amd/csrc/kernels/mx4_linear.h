@@ -43,6 +43,11 @@ __device__ __forceinline__ int mx4_segment(const Mx4Blocks& bl, int nseg, int64_
   return seg;
 }
 
+// A launch holds fewer than 2^32 threads.
+inline bool mx4_launch_ok(int64_t blocks, int threads) {
+  return blocks <= 0xffffffffll / threads;
+}
+
 __device__ __forceinline__ float mx4_silu_mul(float g, float u) {
   return g * (1.0f / (1.0f + expf(-g))) * u;
 }

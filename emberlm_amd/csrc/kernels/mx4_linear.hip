@@ -11,6 +11,9 @@ namespace {
 // Rows of x that a call takes: counted in 31 bits.
 bool rows_ok(int64_t M, int64_t K) { return M >= 0 && M <= 0x7fffffff && mx4_sizes_ok(0, K); }
 
+// Columns of a SwiGLU input half: of few rows, 32 a workgroup of 512 threads.
+constexpr int64_t kMostInner = int64_t(1) << 27;
+
 // The parts of a call that do not depend on its kind.
 Mx4Call call_of(const float* x, int64_t M, int64_t K, const float* norm_w, float eps) {
   Mx4Call c{};
@@ -67,7 +70,7 @@ extern "C" int ember_mx4_gateup(const float* x, int64_t M, int64_t K, const floa
                                 float eps, const void* gate_codes, const void* gate_scales,
                                 const void* up_codes, const void* up_scales, int64_t I, float* out,
                                 void* workspace, size_t workspace_bytes, ember_stream_t s) {
-  if (!rows_ok(M, K) || I < 1 || !mx4_sizes_ok(I, K)) return EMBER_EINVAL;
+  if (!rows_ok(M, K) || I < 1 || I > kMostInner || !mx4_sizes_ok(I, K)) return EMBER_EINVAL;
   if (M == 0) return EMBER_OK;
   if (!x || !gate_codes || !gate_scales || !up_codes || !up_scales || !out) return EMBER_EINVAL;
   for (const void* p : {gate_codes, gate_scales, up_codes, up_scales})

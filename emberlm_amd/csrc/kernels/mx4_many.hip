@@ -14,8 +14,9 @@
 // mx4_split_kernel cuts x into digits once a call, times the norm's weight
 // where there is one, in the form of the matrix cores' operand: a tile of 32 rows
 // by 64 columns is, for each digit, 64 lanes of 16 bytes and then 64 of 8 (two such
-// tiles, 15 KB, lie together: whole copies of 1 KB); scales lie as the weights' do.  It also leaves each row's sums of squares (per 256
-// columns) from which the product's store takes the norm's factor.
+// tiles, 15 KB, lie together: whole copies of 1 KB); scales lie as the weights' do.
+// It also leaves each row's sums of squares (per 256 columns) from which the
+// product's store takes the norm's factor.
 //
 // Sums: a digit's products and their sums of 64 are exact in the MFMA (8 bits,
 // whole numbers of one unit a group); what it adds to is a running fp32 sum, and
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(kSplitThreads) void mx4_split_kernel(Mx4Call c, Spa
       const int byte = top >= 0x7f800000u ? 255 : max(static_cast<int>(top >> 23), 23);
       f32x4 t;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = __builtin_ldexpf(v[h][e], 130 - byte);
+      for (int e = 0; e < 4; ++e) t[e] = byte == 255 ? 0.f : __builtin_ldexpf(v[h][e], 130 - byte);
       const int64_t mb = m / 32;
       const int lane = 32 * h + static_cast<int>(m % 32);
       uint8_t* tile = sp.digits + ((mb / 2 * c.kb + kb) * 2 + mb % 2) * kTileBytes;
@@ -549,7 +550,7 @@ int launch_small(const Mx4Call& c, const Space& sp, hipStream_t st) {
   for (int i = 0; i < c.nseg; ++i) bl.first[i + 1] = bl.first[i] + mx4_row_tiles(c.N[i]);
   const int64_t cols = bl.first[GATE ? 1 : c.nseg], rows = mx4_row_tiles(c.M);
   const int64_t splits = small_splits(cols * rows, c.kb);
-  if (cols * rows * splits > 0x7fffffff) return EMBER_EINVAL;
+  if (!mx4_launch_ok(cols * rows * splits, kSmallWaves * kWave)) return EMBER_EINVAL;
   mx4_small_kernel<GATE><<<static_cast<unsigned>(cols * rows * splits), kSmallWaves * kWave, 0,
                            st>>>(c, sp, bl, static_cast<unsigned>(cols),
                                  static_cast<int>(splits));
@@ -567,7 +568,7 @@ int launch_gemm(const Mx4Call& c, const Space& sp, hipStream_t st) {
     bl.first[i + 1] = bl.first[i] + (mx4_row_tiles(c.N[i]) + S::kOutTiles - 1) / S::kOutTiles;
   const int64_t cols = bl.first[S::GATE ? 1 : c.nseg];
   const int64_t rows = (mx4_row_tiles(c.M) + S::WM - 1) / S::WM;
-  if (cols * rows > 0x7fffffff) return EMBER_EINVAL;
+  if (!mx4_launch_ok(cols * rows, S::kThreads)) return EMBER_EINVAL;
   mx4_gemm_kernel<S><<<static_cast<unsigned>(cols * rows), S::kThreads, 0, st>>>(c, sp, bl,
                                                                   static_cast<unsigned>(cols));
   return launch_status();

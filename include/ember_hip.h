@@ -471,13 +471,20 @@ int ember_mx4_embedding(const int64_t* ids, const void* codes, const void* scale
  * (+ residual[i] [M, N[i]] where residual and residual[i] are not NULL; y[i] may be
  * residual[i]), xn = x where norm_w is NULL, else RMSNorm(x) with weight
  * norm_w [K] and eps.  ember_mx4_gateup: out [M, I] = silu(xn Wg^T) * (xn Wu^T).
- * The codes enter the products as they are held, xn (before the norm's 1 / rms)
- * as whole multiples of at most 2^-23 of the largest size in its group of 32 (and of
- * 2^-127, no less); sums are fp32.  A row of x that is not finite throughout gives
- * a row that is finite nowhere.
+ * Outputs overlap neither x nor each other (EMBER_EINVAL is not given for it).
+ * The codes enter the products as they are held, x (times the norm's weight; its
+ * 1 / rms follows the sum) as whole multiples of at most 2^-23 of the largest size in
+ * its group of 32 columns, and of no less than 2^-127: rounded by at most 2^-24 of
+ * that size, as fp32 values of one exponent.  Sums are fp32.  A row of x (times the
+ * norm's weight) that is not finite throughout gives a row that is finite nowhere;
+ * with a norm, rows' squares have to add up to a finite fp32 as in ember_rmsnorm_fwd.
  * `workspace` >= ember_mx4_workspace_bytes(M, K, rows of all the call's weights)
  * (0: none needed; EMBER_EWORKSPACE when smaller), 256-byte aligned (EMBER_EALIGN).
- * Host arrays are read at the call.  Deterministic. */
+ * A workspace is one call's at a time: calls that may run at once (on two streams,
+ * in two graphs) take one each.  More threads than a launch holds (SwiGLU input halves
+ * of I > 2^27) are refused, EMBER_EINVAL.  Host arrays are read at the call.
+ * Deterministic: the same call gives the same bits (a row's may differ beside another
+ * number of rows). */
 size_t ember_mx4_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int ember_mx4_linear(const float* x, int64_t M, int64_t K, const float* norm_w, float eps,
                      int nseg, const void* const* codes, const void* const* scales,

@@ -113,6 +113,14 @@ def held(r, N, K):
     return dev(c), dev(s), val
 
 
+def held_by_kernel(r, N, K):
+    """The same by the two kernels, which test_store_and_read_back holds to it bit for bit."""
+    c, s = quantize(dev(weight(r, N, K)), N, K)
+    back = empty((N, K))
+    call("ember_mx4_dequantize", p(c), p(s), p(back), N, K, None)
+    return c, s, host(back).astype(np.float64)
+
+
 def workspace(M, K, N):
     need = capi.lib().ember_mx4_workspace_bytes(M, K, N)
     return (raw(need) if need else None), need
@@ -155,9 +163,9 @@ def gateup(x, M, K, g, u, I, norm=None):
     return h
 
 
-def check_product(got, xn, val, extra=None):
+def check_product(got, xn, val, extra=None, floor=0.0):
     y = xn @ val.T
-    bound = OM.product_bound(xn, val, y)
+    bound = OM.product_bound(xn, val, y) + floor
     if extra is not None:
         y = y + extra
         bound = bound + 2.0 ** -24 * np.abs(y)
@@ -182,13 +190,31 @@ LINEAR = [
 ]
 
 
-@pytest.mark.parametrize("M,K,N,norm,res", LINEAR)
+# Sizes that take what those do not, by the workgroups that they make: for few rows two and four
+# tiles of columns a workgroup, and streams of them (K to 1024 and to 2048, one to three rows of tiles);
+# sixteen waves; a K that several workgroups share; tiles of 64 x 128 (K of 1 to 16 tiles) and of 128 x 256
+LARGER = [
+    (2, 300, (9000,), True, True), (6, 1100, (6000, 3000), True, False), (8, 700, (5000,), False, True),
+    (3, 600, (17000,), True, True), (8, 1000, (9000,), True, False), (1, 2100, (33000,), False, True),
+    (1, 576, (20000, 13000), True, True), (3, 1030, (33000,), True, False), (2, 64, (33001, 7), False, True),
+    (5, 250, (17000,), True, True), (6, 2048, (16500, 700), True, False), (7, 1001, (17000,), False, True),
+    (8, 576, (20000, 100, 9000), True, True), (1, 8192, (50, 20), True, True), (3, 4100, (100,), True, True),
+    (2, 3841, (4096,), False, False),
+    (9, 4096, (40,), True, True), (40, 6200, (100, 33), False, True), (20, 8200, (70,), True, False),
+    (700, 37, (4100,), True, True), (900, 100, (3000, 2100), True, False), (600, 190, (4100, 33), False, True),
+    (640, 256, (4000,), True, True), (4000, 260, (4090,), False, False), (1921, 1001, (3900, 150), True, True),
+    (1500, 333, (2100, 2100), True, True), (3900, 450, (2048,), True, False), (2000, 900, (4096,), False, True),
+    (1100, 1600, (4000,), True, True),
+]
+
+
+@pytest.mark.parametrize("M,K,N,norm,res", LINEAR + LARGER)
 def test_linear(M, K, N, norm, res):
     r = rng(M + K + sum(N))
     x = activations(r, M, K)
     nw = (1 + 0.1 * r.standard_normal(K)).astype(np.float32) if norm else None
     xn = OM.rms_norm(x, nw, EPS) if norm else x.astype(np.float64)
-    weights = [held(r, n, K) for n in N]
+    weights = [held(r, n, K) if n < 1000 else held_by_kernel(r, n, K) for n in N]
     rs = [r.standard_normal((M, n)).astype(np.float32) for n in N] if res else None
     y = linear(dev(x), M, K, weights, N, dev(nw) if norm else None,
                [dev(v) for v in rs] if res else None)
@@ -200,14 +226,20 @@ GATEUP = [(1, 1, 1, False), (1, 576, 1536, True), (2, 100, 33, True), (3, 2048, 
           (5, 8192, 40, False), (8, 1001, 65, True), (9, 64, 16, False), (33, 577, 130, True),
           (64, 2048, 129, True), (130, 300, 257, True), (509, 576, 700, True), (600, 1026, 96, False)]
 
+# As LARGER: four tiles a workgroup, a shared K, tiles of 64 x 128 and of 128 x 256
+LARGER_GATEUP = [(3, 700, 8300, True), (6, 1100, 8200, False), (8, 300, 4200, True), (2, 2100, 8300, True),
+                 (33, 4200, 50, True), (12, 9000, 40, False), (700, 37, 4100, True), (900, 192, 2100, False),
+                 (1030, 333, 1900, True), (520, 1001, 1500, True), (2048, 449, 2040, True),
+                 (2048, 1200, 2040, False), (2000, 1030, 2048, True), (4000, 1300, 1020, True)]
 
-@pytest.mark.parametrize("M,K,I,norm", GATEUP)
+
+@pytest.mark.parametrize("M,K,I,norm", GATEUP + LARGER_GATEUP)
 def test_gateup(M, K, I, norm):
     r = rng(M + K + I)
     x = activations(r, M, K)
     nw = (1 + 0.1 * r.standard_normal(K)).astype(np.float32) if norm else None
     xn = OM.rms_norm(x, nw, EPS) if norm else x.astype(np.float64)
-    g, u = held(r, I, K), held(r, I, K)
+    g, u = [(held if I < 1000 else held_by_kernel)(r, I, K) for _ in range(2)]
     h = host(gateup(dev(x), M, K, g, u, I, dev(nw) if norm else None)).astype(np.float64)
     yg, yu = xn @ g[2].T, xn @ u[2].T
     dg, du = OM.product_bound(xn, g[2], yg), OM.product_bound(xn, u[2], yu)
@@ -250,6 +282,81 @@ def test_rows_of_many_sizes_do_not_meet(M):
         assert not np.isfinite(got[bad]).any()  # inf w or NaN, as the sums come
         rest = np.setdiff1d(np.arange(M), bad)
         assert np.array_equal(got[rest], alone[rest])
+
+
+@pytest.mark.parametrize("M", [1, 8, 9, 64, 300])
+@pytest.mark.parametrize("size", [2.0 ** 120, 2.0 ** 90, 2.0 ** -90, 2.0 ** -115])
+def test_ends_of_the_range(M, size):
+    """x near fp32's ends, weights on the other side of 1: products of ordinary size."""
+    r = rng(M)
+    K, N = 256, 70
+    x = (size * np.clip(r.standard_normal((M, K)), -3, 3)).astype(np.float32)
+    w = (r.standard_normal((N, K)) / min(size, 2.0 ** 110) if size > 1 else
+         r.standard_normal((N, K)) * min(1 / size, 2.0 ** 110)).astype(np.float32)
+    c, s, val = OM.hold(w)
+    # x enters in whole multiples of at least 2^-127: a term may be off by 2^-128 |w| beside
+    # product_bound's, which counts steps relative to a group's largest size
+    check_product(linear(dev(x), M, K, [(dev(c), dev(s))], (N,))[0], x.astype(np.float64), val,
+                  floor=2.0 ** -128 * np.abs(val).sum(1))
+
+
+def test_x_in_pieces():
+    """A long x is taken in pieces of rows: K = 65536 in 1024 at a time."""
+    r = rng(3)
+    M, K, N = 1100, 65536, 33
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    x = torch.randn((M, K), generator=gen, device="cuda")
+    assert capi.lib().ember_mx4_workspace_bytes(M, K, N) < 4.5 * 1100 * K  # not all of it at once
+    w = held(r, N, K)
+    nw = dev((1 + 0.1 * r.standard_normal(K)).astype(np.float32))
+    rs = r.standard_normal((M, N)).astype(np.float32)
+    y = linear(x, M, K, [w], (N,), nw, [dev(rs)])[0]
+    rows = [0, 1, 1023, 1024, 1025, 1099]
+    xn = OM.rms_norm(host(x[rows]), host(nw), EPS)
+    check_product(y[rows], xn, w[2], rs[rows])
+
+
+def test_outputs_past_32_bit_offsets():
+    M, K, N = 66000, 33, 33000
+    r = rng(4)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(2)
+    x = torch.randn((M, K), generator=gen, device="cuda")
+    w = held(r, N, K)
+    y = empty((M, N))
+    assert y.numel() > 2 ** 31
+    ws, need = workspace(M, K, N)
+    call("ember_mx4_linear", p(x), M, K, None, EPS, 1, ptrs([w[0]]), ptrs([w[1]]),
+         (C.c_int64 * 1)(N), ptrs([y]), None, p(ws), need, None)
+    rows = [0, 1, 32767, 65073, 65074, 65075, 65998, 65999]
+    check_product(y[rows], host(x[rows]).astype(np.float64), w[2])
+
+
+def test_weights_past_32_bit_offsets():
+    """4.5e9 values: 18 GB of fp32, 2.3 GB of codes."""
+    N, K = 1100000, 4096
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+    w = torch.empty((N, K), device="cuda")
+    for part in w.split(100000):
+        part.copy_(0.02 * torch.randn(part.shape, generator=gen, device="cuda"))
+    codes, scales = quantize(w, N, K)
+    assert codes.numel() > 2 ** 31
+    ids = np.array([0, 31, 32, 524287, 524288, 1048575, 1048576, N - 1])
+    val = OM.hold(host(w[ids]))[2]
+    out, dids = empty((len(ids), K)), dev(ids)
+    call("ember_mx4_embedding", p(dids), p(codes), p(scales), p(out), len(ids), K, N, None)
+    assert np.array_equal(host(out), val.astype(np.float32))
+    w.zero_()
+    call("ember_mx4_dequantize", p(codes), p(scales), p(w), N, K, None)
+    assert np.array_equal(host(w[ids]), val.astype(np.float32))
+    del w
+    r = rng(6)
+    for M in (1, 3, 6, 8, 9, 40):
+        x = activations(r, M, K)
+        y = linear(dev(x), M, K, [(codes, scales)], (N,))[0]
+        check_product(y[:, ids], x.astype(np.float64), val)
 
 
 @pytest.mark.parametrize("M", [1, 8, 9, 300])
@@ -362,13 +469,13 @@ def test_calls_on_two_streams():
         assert np.array_equal(host(y), want)
 
 
-@pytest.mark.parametrize("M", [1, 8, 40, 300])
-def test_captured_and_replayed(M):
+@pytest.mark.parametrize("M,K,I", [(1, 576, 320), (8, 576, 320), (40, 576, 320), (300, 576, 320),
+                                   (1, 600, 17000), (20, 4200, 4300), (2000, 1030, 2048)])
+def test_captured_and_replayed(M, K, I):
     """A block's products in a graph, replayed on new inputs between eager calls."""
     r = rng(M)
-    K, I = 576, 320
     nw = dev((1 + 0.1 * r.standard_normal(K)).astype(np.float32))
-    g, u, d = held(r, I, K), held(r, I, K), held(r, K, I)
+    g, u, d = [held_by_kernel(r, *s) for s in ((I, K), (I, K), (K, I))]
     x, h, y = empty((M, K)), empty((M, I)), empty((M, K))
     ws1, need1 = workspace(M, K, 2 * I)
     ws2, need2 = workspace(M, I, K)

@@ -93,6 +93,9 @@ def test_sizes_are_refused():
         assert lib.ember_mx4_embedding(P, P, P, P, M, 64, 8, None) == -1
         assert lib.ember_mx4_workspace_bytes(M, 64, 64) == 0
     assert _linear(N=(0,)) == -1 and _gateup(N=0) == -1
+    # more threads than a launch holds
+    assert _gateup(M=0, N=2 ** 27) == 0 and _gateup(M=0, N=2 ** 27 + 1) == -1
+    assert _linear(M=1, K=2049, N=(2 ** 31 - 1,)) == -1
     for n in (0, 4, -1):
         assert _linear(nseg=n) == -1
     assert lib.ember_mx4_code_bytes(2 ** 31 - 1, 2 ** 30) == 2 ** 26 * 2 ** 24 * 1024
