@@ -98,6 +98,7 @@ int64_t check_product(const Tensor& x, const Tensor& norm_w,
   if (norm_w.defined()) {
     check_f32(norm_w, op, "norm weight");
     require(norm_w.numel() == K, o + ": norm weight size != in_features");
+    require(!autograd::any_requires_grad({norm_w}), o + ": the norm's weight requires grad");
   }
   return x.numel() / K;
 }

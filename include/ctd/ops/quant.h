@@ -40,7 +40,8 @@ Tensor dequantize_mx4(const Mx4Weight& w);
 // Rows of the table: ids int64 [...] -> fp32 [..., K] (zeros for ids outside it).
 Tensor embedding_mx4(const Tensor& ids, const Mx4Weight& table);
 // Products with such weights, for x [..., K] of any number of rows; none of them
-// records autograd history, and an x that requires grad is refused.
+// records autograd history, and an x, norm weight or residual that requires grad is
+// refused.
 // linear_mx4: for each of 1 to 3 weights, xn W_i^T (+ residuals[i] where given and
 // defined, same shape) -> [..., N_i], xn = RMSNorm(x; norm_w, eps) when norm_w is
 // defined, else x.  gate_up_mx4: silu(xn Wg^T) * (xn Wu^T), the MLP's input half.

@@ -168,6 +168,10 @@ void refusals() {
   Tensor r = randn({2, 8}, 4);
   r.requires_grad_(true);
   refuses([&] { ops::linear_mx4(x, Tensor{}, 0.0f, {&q}, {r}); }, "residual requires grad");
+  Tensor nw = randn({64}, 5);
+  nw.requires_grad_(true);
+  refuses([&] { ops::linear_mx4(x, nw, 1e-5f, {&q}); }, "norm's weight requires grad");
+  refuses([&] { ops::gate_up_mx4(x, nw, 1e-5f, q, q); }, "norm's weight requires grad");
 }
 
 nn::Model small_model(bool qk_norm) {
