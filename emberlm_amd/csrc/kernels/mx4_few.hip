@@ -21,6 +21,7 @@
 // its own LDS, so that no wave waits for another before the sums are joined.
 // A norm's factor 1 / rms is the row's, so it waits for the end: the products
 // take x times the norm's weight.
+#include <algorithm>
 #include <type_traits>
 
 #include "mx4_linear.h"
@@ -73,8 +74,9 @@ __device__ __forceinline__ f32x4 load_x(const float* __restrict__ row, int64_t c
   return v;
 }
 
-// One lane's operand of NT tiles of 16 weight rows by 256 columns, with the
-// scales' bytes for its half of the groups in bytes 0 and 2.
+// One lane's operand of NT tiles of 16 weight rows by 256 columns; a word of scales
+// holds the bytes for its half of the groups at bits 8 (g / 2) and 16 above.  (Shifted
+// when used: a shift behind the load would wait for it.)
 template <int NT>
 struct Operand {
   u32x4 code[NT][2];
@@ -93,12 +95,11 @@ __device__ __forceinline__ void load_weights(Operand<NT>& o, const Mx4Weight (&W
     const int at = 32 * (g & 1) + 16 * (tile[t] & 1) + n;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int64_t k = 4 * kblk + 2 * s + (g >> 1);
-      o.code[t][s] = k < kb ? *reinterpret_cast<const u32x4*>(W[t].codes +
-                                                              ((nb * kb + k) * 64 + at) * 4)
-                            : u32x4{0, 0, 0, 0};
+      // Past the end the last tile again: x's digits are 0 there.
+      const int64_t k = std::min(4 * kblk + 2 * s + (g >> 1), kb - 1);
+      o.code[t][s] = *reinterpret_cast<const u32x4*>(W[t].codes + ((nb * kb + k) * 64 + at) * 4);
     }
-    o.scale[t] = W[t].scales[(nb * ks + kblk) * 64 + at] >> (8 * (g >> 1));
+    o.scale[t] = W[t].scales[(nb * ks + kblk) * 64 + at];
   }
 }
 
@@ -177,16 +178,18 @@ __device__ __forceinline__ Rows read_rows(const uint8_t* mine, const uint8_t* sc
 template <int TT, int NT>
 __device__ __forceinline__ void multiply(f32x4 (&acc)[TT][NT], const Rows& a, int tt,
                                          const Operand<NT>& w, int s) {
+  const int shift = 8 * ((threadIdx.x & (kWave - 1)) >> 5);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
+    const int scale = static_cast<int>(w.scale[t] >> shift);
     const u32x4 q = w.code[t][s];
     const i32x8 b = {(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
     if (s == 0)
       acc[tt][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          a.digits, b, acc[tt][t], 0, 4, 0, a.scale, 0, static_cast<int>(w.scale[t]));
+          a.digits, b, acc[tt][t], 0, 4, 0, a.scale, 0, scale);
     else
       acc[tt][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          a.digits, b, acc[tt][t], 0, 4, 0, a.scale, 2, static_cast<int>(w.scale[t]));
+          a.digits, b, acc[tt][t], 0, 4, 0, a.scale, 2, scale);
   }
 }
 
