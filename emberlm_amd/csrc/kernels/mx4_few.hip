@@ -65,15 +65,6 @@ __device__ __forceinline__ float sum_of_64(float v) {
 // lane's read over another lane's write.
 __device__ __forceinline__ void wave_lds_order() { asm volatile("" ::: "memory"); }
 
-__device__ __forceinline__ f32x4 load_x(const float* __restrict__ row, int64_t c, int64_t K,
-                                        bool vec) {
-  if (vec) return c < K ? *reinterpret_cast<const f32x4*>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
-  f32x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = c + e < K ? row[c + e] : 0.f;
-  return v;
-}
-
 // One lane's operand of NT tiles of 16 weight rows by 256 columns; a word of scales
 // holds the bytes for its half of the groups at bits 8 (g / 2) and 16 above.  (Shifted
 // when used: a shift behind the load would wait for it.)
@@ -112,26 +103,48 @@ struct Shared {
   float squares[W][kMx4FewRows];
 };
 
+// A lane's four columns of x's rows, and of the norm's weight: of rows and columns past
+// the end the last ones, so that no load waits for a branch.
+template <int TT>
+struct Columns {
+  f32x4 x[TT * kTokens], nw;
+};
+template <int TT, bool VEC>
+__device__ __forceinline__ void load_columns_as(const Mx4Call& c, int64_t col, Columns<TT>& o) {
+  const auto load = [&](const float* __restrict__ row) {
+    if constexpr (VEC) return *reinterpret_cast<const f32x4*>(row + std::min(col, c.K - 4));
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = row[std::min(col + e, c.K - 1)];
+    return v;
+  };
+#pragma unroll
+  for (int m = 0; m < TT * kTokens; ++m) o.x[m] = load(c.x + std::min<int64_t>(m, c.M - 1) * c.K);
+  o.nw = load(c.norm_w ? c.norm_w : c.x);
+}
+template <int TT>
+__device__ __forceinline__ void load_columns(const Mx4Call& c, int64_t kblk, Columns<TT>& o) {
+  const int64_t col = kblk * kBlockCols + 4 * (threadIdx.x & (kWave - 1));
+  if (c.x_vec) load_columns_as<TT, true>(c, col, o);
+  else load_columns_as<TT, false>(c, col, o);
+}
+
 // Cuts 256 columns of x's rows (times the norm's weight) into digits in the wave's
 // part of LDS; adds up the rows' squares in ss.
 template <int TT>
-__device__ __forceinline__ void cut_x(const Mx4Call& c, int64_t kblk, uint8_t* mine,
-                                      uint8_t* scale, float (&ss)[TT * kTokens]) {
+__device__ __forceinline__ void cut_x(const Mx4Call& c, int64_t kblk, const Columns<TT>& in,
+                                      uint8_t* mine, uint8_t* scale, float (&ss)[TT * kTokens]) {
   const int lane = threadIdx.x & (kWave - 1), M = static_cast<int>(c.M);
   const int64_t col = kblk * kBlockCols + 4 * lane;
-  f32x4 xv[TT * kTokens];
-#pragma unroll
-  for (int m = 0; m < TT * kTokens; ++m)
-    xv[m] = m < M ? load_x(c.x + m * c.K, col, c.K, c.x_vec) : f32x4{0.f, 0.f, 0.f, 0.f};
-  f32x4 nw{1.f, 1.f, 1.f, 1.f};
-  if (c.norm_w) nw = load_x(c.norm_w, col, c.K, c.x_vec);
 #pragma unroll
   for (int m = 0; m < TT * kTokens; ++m) {
     if (m >= M) continue;
-    f32x4 t = xv[m];
+    f32x4 t;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = col + e < c.K ? in.x[m][e] : 0.f;
     if (c.norm_w) {
       ss[m] += t.x * t.x + t.y * t.y + t.z * t.z + t.w * t.w;
-      t *= nw;
+      t *= in.nw;
     }
     unsigned top = 0;
 #pragma unroll
@@ -296,13 +309,20 @@ __global__ __launch_bounds__(W* kWave) void mx4_few_kernel(Mx4Call c, Mx4Blocks 
   block_tiles<NT, GATE>(c, seg, blk, weight, tile);
   f32x4 acc[TT][NT] = {};
   float ss[TT * kTokens] = {};
+  Columns<TT> x;
   Operand<NT> next;
-  if (w < c.ks) load_weights<NT>(next, weight, tile, w, c.kb, c.ks);
+  if (w < c.ks) {
+    load_columns<TT>(c, w, x);
+    load_weights<NT>(next, weight, tile, w, c.kb, c.ks);
+  }
   for (int64_t kblk = w; kblk < c.ks; kblk += W) {
-    const Operand<NT> cur = next;
     wave_lds_order();  // over the digits of the 256 columns before
-    cut_x<TT>(c, kblk, sh.digits[w], sh.scale[w], ss);
-    if (kblk + W < c.ks) load_weights<NT>(next, weight, tile, kblk + W, c.kb, c.ks);
+    cut_x<TT>(c, kblk, x, sh.digits[w], sh.scale[w], ss);
+    const Operand<NT> cur = next;
+    if (kblk + W < c.ks) {
+      load_columns<TT>(c, kblk + W, x);
+      load_weights<NT>(next, weight, tile, kblk + W, c.kb, c.ks);
+    }
     wave_lds_order();
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -335,8 +355,10 @@ __global__ __launch_bounds__(W* kWave) void mx4_stream_kernel(Mx4Call c, Mx4Bloc
   block_tiles<NT, false>(c, seg, blk, weight, tile);
   Operand<NT> next;
   if (busy) {
+    Columns<TT> x;
+    load_columns<TT>(c, w, x);
     load_weights<NT>(next, weight, tile, w, c.kb, c.ks);
-    cut_x<TT>(c, w, sh.digits[w], sh.scale[w], ss);
+    cut_x<TT>(c, w, x, sh.digits[w], sh.scale[w], ss);
     wave_lds_order();
 #pragma unroll
     for (int s = 0; s < 2; ++s)
