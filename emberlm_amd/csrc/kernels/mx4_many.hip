@@ -148,6 +148,20 @@ __global__ __launch_bounds__(kSplitThreads) void mx4_split_kernel(Mx4Call c, Spa
   }
 }
 
+// A row's factor 1 / rms from its squares, eight loads at a time.
+__device__ __forceinline__ float row_factor(const Mx4Call& c, const Space& sp, int64_t m) {
+  const float* at = sp.squares + m * c.ks;
+  float sum = 0.f;
+  for (int64_t k = 0; k < c.ks; k += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = at[std::min(k + j, c.ks - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += k + j < c.ks ? v[j] : 0.f;
+  }
+  return 1.0f / sqrtf(sum / static_cast<float>(c.K) + c.eps);
+}
+
 // A workgroup's WM x WN waves take 32 rows by 32 TN columns each.  Tiles go from
 // global memory to LDS without registers, a ring of four stages of a tile of K
 // each, two to three ahead, one barrier a stage.
@@ -360,10 +374,7 @@ __global__ __launch_bounds__(S::kThreads) void mx4_gemm_kernel(Mx4Call c, Space 
   // Lane: column lane % 32 of a tile, rows 8 (i / 4) + 4 (lane / 32) + i % 4.
   const int64_t m0 = (int64_t(mt) * S::WM + wm) * 32;
   if (c.norm_w) {
-    const int64_t m = std::min(m0 + lane % 32, c.M - 1);
-    float sum = 0.f;
-    for (int64_t k = 0; k < c.ks; ++k) sum += sp.squares[m * c.ks + k];
-    const float rstd = 1.0f / sqrtf(sum / static_cast<float>(c.K) + c.eps);
+    const float rstd = row_factor(c, sp, std::min(m0 + lane % 32, c.M - 1));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float f = __shfl(rstd, 8 * (i / 4) + 4 * (lane / 32) + i % 4, kWave);
@@ -466,12 +477,8 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c
   for (int t = 0; t < TN; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) red[w][t][i][lane] = hi[t][i] + lo[t][i];
-  if (c.norm_w && threadIdx.x < 32) {
-    const int64_t m = std::min(mb * 32 + lane, c.M - 1);
-    float sum = 0.f;
-    for (int64_t k = 0; k < c.ks; ++k) sum += sp.squares[m * c.ks + k];
-    factor[lane] = 1.0f / sqrtf(sum / static_cast<float>(c.K) + c.eps);
-  }
+  if (c.norm_w && threadIdx.x < 32)
+    factor[lane] = row_factor(c, sp, std::min(mb * 32 + lane, c.M - 1));
   __syncthreads();
   // Two of the 16 accumulator registers a wave; the waves' parts in their order.
   float sum[2][TN];
@@ -526,9 +533,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(Mx4Call c, Space sp, Mx4B
     for (int t = 0; t < TN; ++t)
       v[t] += sp.parts[((static_cast<size_t>(tile) * splits + u) * TN + t) * 1024 + i * 64 + lane];
   if (c.norm_w) {
-    float sum = 0.f;
-    for (int64_t k = 0; k < c.ks; ++k) sum += sp.squares[m * c.ks + k];
-    const float rstd = 1.0f / sqrtf(sum / static_cast<float>(c.K) + c.eps);
+    const float rstd = row_factor(c, sp, m);
 #pragma unroll
     for (int t = 0; t < TN; ++t) v[t] *= rstd;
   }
