@@ -17,10 +17,15 @@
 //
 // A wave takes 256 columns (one register of scales a lane) of 16 NT weight rows
 // at a time, the waves of a workgroup every 256 columns in turn.  It asks for
-// its weights first and cuts up x while they come; its part of x goes through
-// its own LDS, so that no wave waits for another before the sums are joined.
-// A norm's factor 1 / rms is the row's, so it waits for the end: the products
-// take x times the norm's weight.
+// its x and then its weights (loads come back in order), and cuts up x while the
+// weights come; its part of x goes through its own LDS, so that no wave waits for
+// another before the sums are joined.  A norm's factor 1 / rms is the row's, so it
+// waits for the end: the products take x times the norm's weight.
+//
+// In a row of calls: an LM head of 151936 x 2048 32.0 us of one row (5.2 TB/s), 41.1 of
+// eight (cutting x and adding up its digits); the SwiGLU half of 2 x 6144 x 2048 4.9
+// of one row and 10.1 of eight; QKV of 960 x 576 in all 3.5, of which an empty launch
+// takes 2.4.
 #include <algorithm>
 #include <type_traits>
 
