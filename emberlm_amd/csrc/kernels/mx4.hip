@@ -2,7 +2,7 @@
 // into it, read back, and looked up by row.  All three are bound by the fp32
 // side's HBM traffic (4 bytes a value against 17/32): a table of 151936 x 2048 is
 // brought into it in 263-305 us and read back in 259-272 (4.6 to 5.4 TB/s), 4096 of its
-// rows looked up in 12.9 (2.9 TB/s, much of it latency).  The reference holds its weights
+// rows looked up in 12.9 (lines of 128 bytes for runs of 16, mx4_embedding_kernel).  The reference holds its weights
 // in fp32 only.
 #include "mx4.h"
 
@@ -118,33 +118,46 @@ __global__ __launch_bounds__(kThreads) void mx4_dequantize_kernel(
   }
 }
 
-// One wave per (id, 256 columns): lane i takes columns 4 i of the block.  A row
-// of the table lies in runs of 16 bytes, two a tile, so a lookup reads whole
-// 64-byte sectors for them; its bound is the fp32 row that it writes.
-template <bool VEC>
+// One wave per (id, BLOCKS blocks of 256 columns): lane i takes columns 4 i of each.
+// A row of the table lies in runs of 16 bytes, two a tile, and of 4 for the scales, each
+// in a line of 128 that its neighbours share: for 1088 bytes of a row of 2048 columns some
+// 10 KB cross the caches beside the 8 KB that are written.
+template <bool VEC, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void mx4_embedding_kernel(
     const int64_t* __restrict__ ids, const uint16_t* __restrict__ codes,
     const uint8_t* __restrict__ scales, float* __restrict__ out, int64_t n, int64_t K, int64_t V,
     int64_t kb, int64_t ks) {
   const int lane = threadIdx.x & (kWave - 1);
   constexpr int kWaves = kThreads / kWave;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave; it < n * ks;
-       it += static_cast<int64_t>(gridDim.x) * kWaves) {
-    const int64_t i = it / ks, kc = it % ks;
+  const int64_t groups = (ks + BLOCKS - 1) / BLOCKS;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
+       it < n * groups; it += static_cast<int64_t>(gridDim.x) * kWaves) {
+    const int64_t i = it / groups, first = it % groups * BLOCKS;
     const int64_t id = ids[i];
-    const int64_t c = kc * kCols + 4 * lane;
-    if (c >= K) continue;
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
-    if (id >= 0 && id < V) {
-      const int64_t nb = id / 32, r = id % 32, t = lane / 16, h = lane / 8 % 2;
-      const unsigned byte = scales[(nb * ks + kc) * kMx4ScaleBytes + (32 * h + r) * 4 + t];
-      const unsigned code = codes[(nb * kb + kc * 4 + t) * (kMx4TileBytes / 2) + (32 * h + r) * 8 +
-                                  lane % 8];
-      v = mx4_values(code, static_cast<int>(byte));
+    const bool known = id >= 0 && id < V;
+    const int64_t nb = id / 32, r = id % 32;
+    const int t = lane / 16, h = lane / 8 % 2;
+    unsigned byte[BLOCKS], code[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int64_t kc = first + b;
+      byte[b] = code[b] = 0;
+      if (!known || kc * kCols + 4 * lane >= K) continue;
+      byte[b] = scales[(nb * ks + kc) * kMx4ScaleBytes + (32 * h + r) * 4 + t];
+      code[b] = codes[(nb * kb + kc * 4 + t) * (kMx4TileBytes / 2) + (32 * h + r) * 8 + lane % 8];
     }
-    store4<VEC>(out + i * K, c, K, v);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+      store4<VEC>(out + i * K, (first + b) * kCols + 4 * lane, K,
+                  mx4_values(code[b], static_cast<int>(byte[b])));
   }
 }
+
+// A lookup of more blocks than the GPU has room for waves takes two of them a wave, whose
+// loads go out together (32768 rows of K = 2048 113.6 -> 96.0 us, four a wave 97.6; 2048
+// rows 8.1 -> 7.5, and 8.5).
+constexpr int kWide = 2;
+constexpr int64_t kManyBlocks = 8192;
 
 bool vec(const float* w, int64_t K) { return K % 4 == 0 && aligned16(w); }
 
@@ -201,8 +214,12 @@ extern "C" int ember_mx4_embedding(const int64_t* ids, const void* codes, const 
   if (!aligned16(codes) || !aligned16(scales)) return EMBER_EALIGN;
   const int64_t kb = mx4_col_tiles(K), ks = mx4_col_blocks(K);
   constexpr int kWaves = kThreads / kWave;
-  auto* kernel = vec(out, K) ? mx4_embedding_kernel<true> : mx4_embedding_kernel<false>;
-  kernel<<<grid_of((n * ks + kWaves - 1) / kWaves), kThreads, 0, as_stream(s)>>>(
+  const bool wide = n * ks >= kManyBlocks;
+  auto* kernel = vec(out, K) ? wide ? mx4_embedding_kernel<true, kWide> : mx4_embedding_kernel<true, 1>
+                 : wide      ? mx4_embedding_kernel<false, kWide>
+                             : mx4_embedding_kernel<false, 1>;
+  const int64_t groups = wide ? (ks + kWide - 1) / kWide : ks;
+  kernel<<<grid_of((n * groups + kWaves - 1) / kWaves), kThreads, 0, as_stream(s)>>>(
       ids, static_cast<const uint16_t*>(codes), static_cast<const uint8_t*>(scales), out, n, K, V,
       kb, ks);
   return launch_status();

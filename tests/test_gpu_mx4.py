@@ -91,11 +91,12 @@ def test_store_and_read_back(N, K, off):
     assert (got[:off] == 3.0).all() and (got[off + N * K:] == 3.0).all()
 
 
-@pytest.mark.parametrize("V,K", [(1, 1), (33, 65), (200, 576), (77, 1001), (5, 300)])
-def test_lookup(V, K):
+@pytest.mark.parametrize("V,K,n", [(1, 1, 40), (33, 65, 40), (200, 576, 40), (77, 1001, 40),
+                                   (5, 300, 40), (40, 700, 3000), (33, 257, 5000), (50, 130, 9000)])
+def test_lookup(V, K, n):
     r = rng(V + K)
     c, s, val = OM.hold(odd_values(weight(r, V, K), r))
-    ids = np.concatenate([r.integers(0, V, 40), [0, V - 1, V - 1, -1, V, 2 ** 40, -2 ** 40]])
+    ids = np.concatenate([r.integers(0, V, n), [0, V - 1, V - 1, -1, V, 2 ** 40, -2 ** 40]])
     want = np.where(((ids >= 0) & (ids < V))[:, None], val[np.clip(ids, 0, V - 1)], 0.0)
     dids, c, s = dev(ids), dev(c), dev(s)
     for off in (0, 1):
