@@ -391,7 +391,21 @@ __global__ __launch_bounds__(S::kThreads) void mx4_gemm_kernel(Mx4Call c, Space 
   }
   constexpr int kOutT = GATE ? S::TN / 2 : S::TN;
   float* y = c.y[seg];
-  const float* res = c.res[seg];
+  if (const float* res = GATE ? nullptr : c.res[seg]) {
+    // All loads before the first store and without branches (past the end of the last row
+    // and column), or each would wait for its own and for the store before it.
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int64_t m = std::min(m0 + 8 * (i / 4) + 4 * (lane / 32) + i % 4, c.M - 1);
+#pragma unroll
+      for (int t = 0; t < kOutT; ++t) {
+        const int64_t n = (nblk * S::kOutTiles + wn * kOutT + t) * 32 + lane % 32;
+        lo[t][i] = res[m * N + std::min(n, N - 1)];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kOutT; ++t) hi[t] += lo[t];
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t m = m0 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
@@ -401,7 +415,7 @@ __global__ __launch_bounds__(S::kThreads) void mx4_gemm_kernel(Mx4Call c, Space 
       const int64_t n = (nblk * S::kOutTiles + wn * kOutT + t) * 32 + lane % 32;
       if (n >= N) continue;
       if constexpr (GATE) y[m * N + n] = mx4_silu_mul(hi[t][i], hi[kOutT + t][i]);
-      else y[m * N + n] = res ? res[m * N + n] + hi[t][i] : hi[t][i];
+      else y[m * N + n] = hi[t][i];
     }
   }
 }
@@ -507,6 +521,15 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c
     return;
   }
   const int64_t N = c.N[seg], n = nblk * 32 + lane % 32;
+  float extra[2] = {};
+  if (const float* res = GATE ? nullptr : c.res[seg]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = 2 * w + j;
+      const int64_t m = std::min(mb * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4, c.M - 1);
+      extra[j] = res[m * N + std::min(n, N - 1)];
+    }
+  }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = 2 * w + j, r = 8 * (i / 4) + 4 * (lane / 32) + i % 4;
@@ -517,7 +540,7 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void mx4_small_kernel(Mx4Call c
     for (int t = 0; t < TN; ++t) v[t] = c.norm_w ? sum[j][t] * factor[r] : sum[j][t];
     float* y = c.y[seg] + m * N + n;
     if constexpr (GATE) *y = mx4_silu_mul(v[0], v[1]);
-    else *y = c.res[seg] ? c.res[seg][m * N + n] + v[0] : v[0];
+    else *y = extra[j] + v[0];
   }
 }
 
