@@ -48,8 +48,19 @@ inline bool mx4_launch_ok(int64_t blocks, int threads) {
   return blocks <= 0xffffffffll / threads;
 }
 
+// silu(g) u.  With q = e^-|g| the sigmoid is 1 / (1 + q), or q / (1 + q) left of 0: nothing
+// overflows, and a reciprocal of 1 to 2 and an exponential whose argument keeps its
+// second word (log2 e in two) are each off by two half steps.  e^g below 2^-126 counts as
+// 0.  (14 instructions for the 36 of expf and a division: 2048 rows to 2 x 6144 columns 149.7
+// -> 145.4 us.)
 __device__ __forceinline__ float mx4_silu_mul(float g, float u) {
-  return g * (1.0f / (1.0f + expf(-g))) * u;
+  constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596303e-8f, kLn2 = 0.693147181f;
+  const float a = fminf(fabsf(g), 200.f);
+  const float t = -kLog2eHi * a;
+  const float rest = __builtin_fmaf(-kLog2eHi, a, -t) - kLog2eLo * a;
+  const float q = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(rest, kLn2, 1.f);
+  const float top = g < 0.f ? g * q : g;
+  return top * __builtin_amdgcn_rcpf(1.f + q) * u;
 }
 
 // Calls of few rows (mx4_few.hip).  Each of its workgroups cuts all of x into digits

@@ -67,7 +67,7 @@ def rms_norm(x, w, eps):
 
 
 def silu(g):
-    return g / (1 + np.exp(-g))
+    return g / (1 + np.exp(np.minimum(-g, 700.0)))
 
 
 def product_bound(x, w, y):

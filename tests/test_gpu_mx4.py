@@ -234,6 +234,33 @@ LARGER_GATEUP = [(3, 700, 8300, True), (6, 1100, 8200, False), (8, 300, 4200, Tr
                  (2048, 1200, 2040, False), (2000, 1030, 2048, True), (4000, 1300, 1020, True)]
 
 
+def check_gateup(h, xn, g, u):
+    yg, yu = xn @ g.T, xn @ u.T
+    dg, du = OM.product_bound(xn, g, yg), OM.product_bound(xn, u, yu)
+    want = OM.silu(yg) * yu
+    # |silu'| <= 1.1; exp's, the quotient's and two products' roundings, of which exp's scales with
+    # the fp32 argument: 2^-23 |g| more; e^g below 2^-126 counts as 0
+    bound = (1.1 * dg * (np.abs(yu) + du) + (np.abs(OM.silu(yg)) + dg) * du +
+             2.0 ** -23 * (6 + np.abs(yg)) * np.abs(want) + 2.0 ** -126 * (1 + np.abs(yg * yu)))
+    err = np.abs(h - want)
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("M,I", [(1, 5000), (8, 300), (9, 300), (600, 2100), (2048, 2040)])
+def test_gates_of_all_sizes(M, I):
+    """Gates from -2000 to 2000 and around 0, upwards of 0 and below where e^-|g| ends."""
+    r = rng(M)
+    K = 64
+    x = activations(r, M, K)
+    size = np.exp2(r.integers(-20, 9, (I, 1)))
+    g, u = [(r.standard_normal((I, K)) * s / 8).astype(np.float32) for s in (size, 1.0)]
+    (gc, gs, gv), (uc, us, uv) = OM.hold(g), OM.hold(u)
+    h = host(gateup(dev(x), M, K, (dev(gc), dev(gs)), (dev(uc), dev(us)), I)).astype(np.float64)
+    yg = x.astype(np.float64) @ gv.T
+    assert yg.min() < -200 and yg.max() > 200
+    check_gateup(h, x.astype(np.float64), gv, uv)
+
+
 @pytest.mark.parametrize("M,K,I,norm", GATEUP + LARGER_GATEUP)
 def test_gateup(M, K, I, norm):
     r = rng(M + K + I)
@@ -242,14 +269,7 @@ def test_gateup(M, K, I, norm):
     xn = OM.rms_norm(x, nw, EPS) if norm else x.astype(np.float64)
     g, u = [(held if I < 1000 else held_by_kernel)(r, I, K) for _ in range(2)]
     h = host(gateup(dev(x), M, K, g, u, I, dev(nw) if norm else None)).astype(np.float64)
-    yg, yu = xn @ g[2].T, xn @ u[2].T
-    dg, du = OM.product_bound(xn, g[2], yg), OM.product_bound(xn, u[2], yu)
-    want = OM.silu(yg) * yu
-    # |silu'| <= 1.1; exp's, the quotient's and two products' roundings, of which exp's scales with
-    # the fp32 argument: 2^-23 |g| more
-    bound = (1.1 * dg * (np.abs(yu) + du) + (np.abs(OM.silu(yg)) + dg) * du +
-             2.0 ** -23 * (6 + np.abs(yg)) * np.abs(want) + 2.0 ** -126)
-    assert (np.abs(h - want) <= bound).all(), (np.abs(h - want) / bound).max()
+    check_gateup(h, xn, g[2], u[2])
 
 
 @pytest.mark.parametrize("M", [1, 5, 8, 9, 40, 300])
