@@ -2,7 +2,7 @@
 // into it, read back, and looked up by row.  All three are bound by the fp32
 // side's HBM traffic (4 bytes a value against 17/32): a table of 151936 x 2048 is
 // brought into it in 263-305 us and read back in 259-272 (4.6 to 5.4 TB/s), 4096 of its
-// rows looked up in 12.9 (lines of 128 bytes for runs of 16, mx4_embedding_kernel).  The reference holds its weights
+// rows looked up in 12.2 (lines of 128 bytes for runs of 16, mx4_embedding_kernel).  The reference holds its weights
 // in fp32 only.
 #include "mx4.h"
 

@@ -24,11 +24,11 @@
 // and digits 2 to 4 have sums of their own, so that the small ones meet no large
 // sum before the end.
 //
-// Measured: 2048 rows of K = 2048 to the SwiGLU half of 2 x 6144 columns 146 us with
-// the norm, of them 12.7 for the digits (704 TFLOP/s in all, 770 in the product); 4096 rows
-// of K = 6144 to 2048 columns 187, of them 42 for the digits (550 and 715).  In the product
-// the matrix cores are busy 47% of the cycles, at a clock of 1.86 GHz that their power sets
-// (zeros run a fifth faster); a round of tiles adds some 10 us before its first and behind
+// Measured: 2048 rows of K = 2048 to the SwiGLU half of 2 x 6144 columns 139-145 us with
+// the norm, of them 12.2 for the digits (730 TFLOP/s in all, 780 in the product); 4096 rows
+// of K = 6144 to 2048 columns 163, of them 42 for the digits (630 and 845).  In the product
+// the matrix cores are busy half of the cycles, at a clock of 1.86 GHz that their power sets
+// (zeros run a fifth faster); a round of tiles adds some 8 us before its first and behind
 // its last product.
 #include <algorithm>
 
@@ -646,7 +646,7 @@ Kernel kernel_of(const Mx4Call& c, bool gate) {
 }
 
 // An x of more values than these is read past the caches, which its digits then have to
-// themselves until the product reads them (4096 x 6144, 100 MB: 195 -> 178 us in all); a
+// themselves until the product reads them (4096 x 6144, 100 MB: 195 -> 178 us when it was built); a
 // smaller one may still be there when the product's residual or the caller wants it (2048 x
 // 6144: 102 us, read past them 105).
 constexpr int64_t kKeep = int64_t(1) << 24;
