@@ -471,7 +471,7 @@ int ember_mx4_embedding(const int64_t* ids, const void* codes, const void* scale
  * (+ residual[i] [M, N[i]] where residual and residual[i] are not NULL; y[i] may be
  * residual[i]), xn = x where norm_w is NULL, else RMSNorm(x) with weight
  * norm_w [K] and eps.  ember_mx4_gateup: out [M, I] = silu(xn Wg^T) * (xn Wu^T).
- * Outputs overlap neither x nor each other (EMBER_EINVAL is not given for it).
+ * Outputs overlap neither x nor each other nor another weight's residual (not checked).
  * The codes enter the products as they are held, x (times the norm's weight; its
  * 1 / rms follows the sum) as whole multiples of at most 2^-23 of the largest size in
  * its group of 32 columns, and of no less than 2^-127: rounded by at most 2^-24 of
