@@ -103,7 +103,7 @@ __device__ __forceinline__ void load_weights(Operand<NT>& o, const Mx4Weight (&W
 template <int TT, int NT, int W>
 struct Shared {
   __attribute__((aligned(16))) uint8_t digits[W][TT * kTileLds];  // and a wave's sums
-  uint8_t scale[W][kMx4FewRows * 8];
+  uint8_t scale[W][TT * kTokens * 8];
   float parts[W][NT][kMx4FewRows][16];
   float squares[W][kMx4FewRows];
 };
@@ -180,10 +180,13 @@ struct Rows {
   i32x8 digits;
   int scale;
 };
-__device__ __forceinline__ Rows read_rows(const uint8_t* mine, const uint8_t* scale, int tt,
+template <int TT, size_t ROOM>
+__device__ __forceinline__ Rows read_rows(const uint8_t* mine, const uint8_t (&scale)[ROOM], int tt,
                                           int s) {
+  static_assert(ROOM >= TT * kTokens * 8, "read for rows of no token too");
   const int lane = threadIdx.x & (kWave - 1), r = lane & 15, g = lane >> 4;
-  // Row 15 of a tile holds nothing that is read again; nor do rows of no token.
+  // Row 15 of a tile holds nothing that is read again; nor do rows of no token, up to TT
+  // kTokens of which are read.
   const int m_of = r < kTokens * kDigits ? r / kDigits : 0, p_of = r % kDigits;
   const uint8_t* row = mine + tt * kTileLds + r * kRowBytes + 128 * s + 16 * g;
   const u32x4 lo = *reinterpret_cast<const u32x4*>(row);
@@ -333,7 +336,7 @@ __global__ __launch_bounds__(W* kWave) void mx4_few_kernel(Mx4Call c, Mx4Blocks 
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt)
-        multiply<TT, NT>(acc, read_rows(sh.digits[w], sh.scale[w], tt, s), tt, cur, s);
+        multiply<TT, NT>(acc, read_rows<TT>(sh.digits[w], sh.scale[w], tt, s), tt, cur, s);
   }
   add_digits<TT, NT>(acc, sh.digits[w], static_cast<int>(c.M), sh.parts[w]);
   note_squares<TT, NT, W>(c, ss, sh, w);
@@ -368,7 +371,7 @@ __global__ __launch_bounds__(W* kWave) void mx4_stream_kernel(Mx4Call c, Mx4Bloc
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int tt = 0; tt < TT; ++tt) rows[s][tt] = read_rows(sh.digits[w], sh.scale[w], tt, s);
+      for (int tt = 0; tt < TT; ++tt) rows[s][tt] = read_rows<TT>(sh.digits[w], sh.scale[w], tt, s);
   }
   note_squares<TT, NT, W>(c, ss, sh, w);
   bool odd = false;
