@@ -4,7 +4,8 @@
   compiled with hipcc for gfx950 only.
 * ``emberlm_amd/lib/libctd.so``        -- the C++ Tensor/autograd/Module/optim layer
   (include/ctd/...), host-only C++ that calls nothing but the C ABI.
-* ``emberlm_amd/lib/ctd_tests``, ``ctd_quant_tests``, ``ctd_mx4_tests`` -- the C++ test binaries (tests/cpp/).
+* ``emberlm_amd/lib/ctd_tests``, ``ctd_quant_tests``, ``ctd_mx4_tests``,
+  ``ctd_mx4_model_tests`` -- the C++ test binaries (tests/cpp/).
 
 Usage: ``python -m emberlm_amd.build`` (or ``__graft_entry__.build()``).
 """
@@ -97,7 +98,8 @@ def build_host(verbose=False):
 
 def build_cpp_tests(verbose=False):
     """The test programs: tests/cpp/*.cpp into lib/ctd_tests, tests/cpp/quant/*.cpp into
-    lib/ctd_quant_tests, tests/cpp/mx4/*.cpp into lib/ctd_mx4_tests."""
+    lib/ctd_quant_tests, tests/cpp/mx4/*.cpp into lib/ctd_mx4_tests, tests/cpp/mx4_model/*.cpp
+    into lib/ctd_mx4_model_tests."""
     if not os.path.exists(os.path.join(LIB, "libctd.so")):
         return []
     cxx = shutil.which("g++") or "g++"
@@ -105,7 +107,7 @@ def build_cpp_tests(verbose=False):
     oracle_lib = os.path.join(ROOT, "oracle", "_build")
     outs = []
     for folder, name in ((".", "ctd_tests"), ("quant", "ctd_quant_tests"),
-                         ("mx4", "ctd_mx4_tests")):
+                         ("mx4", "ctd_mx4_tests"), ("mx4_model", "ctd_mx4_model_tests")):
         srcs = sorted(glob.glob(os.path.join(ROOT, "tests", "cpp", folder, "*.cpp")))
         if not srcs:
             continue

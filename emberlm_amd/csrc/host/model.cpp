@@ -332,9 +332,9 @@ void Model::quantize_weights(bool table) {
                       &b.self_attn.o_proj, &b.mlp.gate_proj, &b.mlp.up_proj, &b.mlp.down_proj})
       hold(l->weight, l->mx4);
   if (table) hold(embed_tokens.weight, embed_tokens.mx4);
-  auto settle = [](Tensor& t) {
-    if (t.defined()) t.requires_grad_(false);
-  };
+  // Handles of their own: a copy of the model, an optimizer or a list of parameters may hold
+  // the same tensors, and their gradients are theirs.
+  auto settle = [](Tensor& t) { t = t.detach(); };
   settle(embed_tokens.weight);
   settle(norm.weight);
   for (TransformerBlock& b : layers)

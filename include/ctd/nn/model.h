@@ -85,7 +85,9 @@ struct Model {
   // values.  forward, forward_last_logits and generation then run on the 4-bit
   // weights; the training forwards give logits and losses without a graph (no
   // tensor of the model requires grad any more), and collect_parameters throws.  A
-  // second call may add the table.
+  // second call may add the table.  Models that were copied from this one, or it from
+  // them, keep their weights and gradients as they are (what stays in fp32, norms and
+  // table, goes on being shared; what another model or list holds is not freed).
   void quantize_weights(bool table = false);
   bool weights_quantized() const { return !layers.empty() && layers[0].mx4(); }
 
