@@ -5,6 +5,7 @@
 #include <stdexcept>
 #include <string>
 
+#include "ctd/allocator.h"
 #include "ctd/ops/decode.h"
 #include "ctd/ops/loss.h"
 #include "ctd/runtime.h"
@@ -341,6 +342,7 @@ void Model::quantize_weights(bool table) {
     for (RMSNorm* n : {&b.input_layernorm, &b.post_attention_layernorm, &b.self_attn.q_norm,
                        &b.self_attn.k_norm})
       settle(n->weight);
+  empty_device_cache();  // or the process would go on holding what the fp32 weights took
 }
 
 Model::NamedParameters Model::collect_parameters() {

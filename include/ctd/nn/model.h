@@ -87,7 +87,8 @@ struct Model {
   // tensor of the model requires grad any more), and collect_parameters throws.  A
   // second call may add the table.  Models that were copied from this one, or it from
   // them, keep their weights and gradients as they are (what stays in fp32, norms and
-  // table, goes on being shared; what another model or list holds is not freed).
+  // table, goes on being shared; what another model or list holds is not freed).  Memory
+  // that became free goes back to the driver.
   void quantize_weights(bool table = false);
   bool weights_quantized() const { return !layers.empty() && layers[0].mx4(); }
 

@@ -23,3 +23,23 @@ def test_cpp_api_tests():
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     print(r.stdout)
     assert r.returncode == 0 and "0 failure(s)" in r.stdout, r.stdout + r.stderr
+
+
+def test_memory_goes_back_to_the_driver():
+    """What the allocator holds shrinks with what lives: beside it, segments that a few 4-bit
+    buffers lie in, each of the size of an fp32 weight (4 MB at most here, 126 MB in all) or of
+    2 MB for the small ones."""
+    c = TR.make_config(vocab_size=512, hidden_size=512, intermediate_size=2048, num_layers=8,
+                       num_heads=4, num_kv_heads=2, head_dim=128, rms_norm_eps=1e-5, rope_theta=1e4)
+    TR.empty_cache()
+    base = TR.memory().reserved
+    tr = TR.Trainer(c, seed=0)
+    before = TR.memory().reserved - base
+    assert before >= 125 * 10 ** 6
+    for table in (False, True):
+        live = TR.memory().allocated
+        tr.quantize_weights(table)
+        m = TR.memory()
+        assert m.allocated < live
+        assert m.reserved - base <= m.allocated + (2 * 4 + 4 * 2 << 20)
+    tr.close()
