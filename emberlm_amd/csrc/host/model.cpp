@@ -323,16 +323,25 @@ Model build_model(const TensorDict& w, const LlamaConfig& cfg) {
 
 void Model::quantize_weights(bool table) {
   autograd::NoGradGuard ng;
-  auto hold = [](Tensor& w, ops::Mx4Weight& mx4) {
-    if (mx4.defined()) return;
-    mx4 = ops::quantize_mx4(w);
-    w = Tensor{};
+  // All of them before the first fp32 weight goes, so that a failure (no memory) changes nothing.
+  struct Held {
+    Tensor* weight;
+    ops::Mx4Weight* to;
+    ops::Mx4Weight mx4;
+  };
+  std::vector<Held> done;
+  auto hold = [&done](Tensor& w, ops::Mx4Weight& to) {
+    if (!to.defined()) done.push_back({&w, &to, ops::quantize_mx4(w)});
   };
   for (TransformerBlock& b : layers)
     for (Linear* l : {&b.self_attn.q_proj, &b.self_attn.k_proj, &b.self_attn.v_proj,
                       &b.self_attn.o_proj, &b.mlp.gate_proj, &b.mlp.up_proj, &b.mlp.down_proj})
       hold(l->weight, l->mx4);
   if (table) hold(embed_tokens.weight, embed_tokens.mx4);
+  for (Held& h : done) {
+    *h.to = std::move(h.mx4);
+    *h.weight = Tensor{};
+  }
   // Handles of their own: a copy of the model, an optimizer or a list of parameters may hold
   // the same tensors, and their gradients are theirs.
   auto settle = [](Tensor& t) { t = t.detach(); };

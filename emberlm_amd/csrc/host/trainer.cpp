@@ -296,13 +296,14 @@ int ctd_trainer_quantize_weights(ctd_trainer_t t, int32_t table) {
     Trainer* tr = as_trainer(t);
     if (tr->opt) tr->opt->wait_idle();
     runtime::synchronize();
+    tr->model.quantize_weights(table != 0);  // throws before it changes anything
+    runtime::synchronize();
     tr->model.recompute_hook = nullptr;
     tr->opt.reset();
     tr->named = {};
     tr->decay.clear();
     tr->opt_index.clear();
-    tr->model.quantize_weights(table != 0);
-    runtime::synchronize();
+    empty_device_cache();  // what those held
   });
 }
 

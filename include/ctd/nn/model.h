@@ -88,7 +88,8 @@ struct Model {
   // second call may add the table.  Models that were copied from this one, or it from
   // them, keep their weights and gradients as they are (what stays in fp32, norms and
   // table, goes on being shared; what another model or list holds is not freed).  Memory
-  // that became free goes back to the driver.
+  // that became free goes back to the driver.  While it runs the 4-bit weights are there
+  // beside all fp32 ones; a failure (no memory for them) changes nothing.
   void quantize_weights(bool table = false);
   bool weights_quantized() const { return !layers.empty() && layers[0].mx4(); }
 

@@ -91,7 +91,7 @@ int ctd_trainer_set_checkpoint_bits(ctd_trainer_t t, int32_t bits);
 /* Holds the model's projections (and, with table != 0, its embedding table and
  * LM head) in 4 bits from here on (Model::quantize_weights): forward, generation
  * and losses run on them.  The handle has no parameters, gradients or optimizer
- * any more: the calls that need them fail. */
+ * any more: the calls that need them fail.  A call that fails changes nothing. */
 int ctd_trainer_quantize_weights(ctd_trainer_t t, int32_t table);
 /* Batch: ids/targets int64 [B,T], mask fp32 [B,T] (NULL = all ones), host memory. */
 int ctd_trainer_set_batch(ctd_trainer_t t, const int64_t* ids, const int64_t* targets,

@@ -3,6 +3,7 @@ gradients, memory."""
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -43,3 +44,33 @@ def test_memory_goes_back_to_the_driver():
         assert m.allocated < live
         assert m.reserved - base <= m.allocated + (2 * 4 + 4 * 2 << 20)
     tr.close()
+
+
+@pytest.mark.parametrize("steps,room", [(0, 0), (0, 16 << 20), (1, 0)])
+def test_a_failure_changes_nothing(steps, room):
+    """No memory for the first 4-bit weight, or for one further on (40 MB are needed)."""
+    c = TR.make_config(vocab_size=512, hidden_size=2048, intermediate_size=4096, num_layers=2,
+                       num_heads=16, num_kv_heads=8, head_dim=128, rms_norm_eps=1e-5, rope_theta=1e4)
+    ids = np.random.default_rng(1).integers(0, 512, (1, 9))
+    losses = []
+    for fails in (False, True):
+        tr = TR.Trainer(c, seed=0)
+        tr.set_batch(ids, ids)
+        if steps:
+            tr.make_optimizer()
+            tr.train_step()
+        if fails:
+            TR.empty_cache()
+            TR.set_memory_limit(TR.memory().reserved + room)
+            try:
+                with pytest.raises(TR.CtdError):
+                    tr.quantize_weights(True)
+            finally:
+                TR.set_memory_limit(0)
+        if not steps:
+            tr.make_optimizer()
+        run = [tr.train_step().loss, tr.forward_backward(False)]
+        tr.quantize_weights(True)
+        losses.append(run + [tr.forward_backward(False)])
+        tr.close()
+    assert losses[0] == losses[1]
