@@ -90,3 +90,38 @@ def product_bound(x, w, y):
     groups = np.sqrt((top * top) @ (w * w).T)
     n = 24 + 2 * -(-K // 64)
     return 2.0 ** -24 * (7 * groups + 7 * terms + n * (np.abs(y) + 7 * terms)) + 2.0 ** -126
+
+
+def rms_bound(x, w, y):
+    """What the error of each element of y = x w^T [M, N] is below in the mean of its square's root.
+
+    The roundings of product_bound, each at most half a step, 2^-24, of its value and independent of
+    each other, so that their squares add up: one a term, of x's group's largest size, and one where a
+    norm's weight is multiplied in; and 24 + K / 64 of running sums (of the upper digits; the lower
+    ones' sums are 2^-9 of these), which are below |y| and the root of their terms' squares.  (A
+    rounding's own mean square is a third of what is counted here.  What the matrix cores drop, below
+    2^-27 of a running sum, is an eighth of a half step a time.)
+    """
+    x, w = np.abs(x), np.abs(w)
+    K = x.shape[1]
+    top = np.repeat(np.maximum.reduceat(x, np.arange(0, K, GROUP), axis=1), GROUP, 1)[:, :K]
+    terms = (x * x) @ (w * w).T
+    groups = (top * top) @ (w * w).T
+    return 2.0 ** -24 * np.sqrt(groups + terms + (24 + K / 64) * (y * y + terms))
+
+
+def gateup_rms_bound(x, g, u):
+    """The same of silu(x g^T) * (x u^T): either factor's error through the product (|silu'| <= 1.1),
+    and six roundings and the exponential's of the result."""
+    yg, yu = x @ g.T, x @ u.T
+    own = 2.0 ** -23 * (6 + np.abs(yg)) * np.abs(silu(yg) * yu)
+    return np.sqrt((1.1 * rms_bound(x, g, yg) * yu) ** 2 + (silu(yg) * rms_bound(x, u, yu)) ** 2 +
+                   own ** 2)
+
+
+def in_digits(x, digits):
+    """x as the first of its base-32 digits: a group's scale is 2^-3 of its largest size's power of two."""
+    K = x.shape[1]
+    top = np.repeat(np.maximum.reduceat(np.abs(x), np.arange(0, K, GROUP), axis=1), GROUP, 1)[:, :K]
+    unit = np.ldexp(1.0, np.frexp(np.where(top > 0, top, 1.0))[1] - 4 - 5 * (digits - 1))
+    return np.rint(x / unit) * unit
