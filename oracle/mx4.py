@@ -97,8 +97,9 @@ def rms_bound(x, w, y):
 
     The roundings of product_bound, each at most half a step, 2^-24, of its value and independent of
     each other, so that their squares add up: one a term, of x's group's largest size, and one where a
-    norm's weight is multiplied in; and 24 + K / 64 of running sums (of the upper digits; the lower
-    ones' sums are 2^-9 of these), which are below |y| and the root of their terms' squares.  (A
+    norm's weight is multiplied in; 24 for the split of K, the norm's factor and the store; and K / 32
+    of running sums, one a group (of the upper digits; the lower ones' sums are 2^-9 of these), which
+    grow up to y and to the root of their terms' squares, their squares half of that on average.  (A
     rounding's own mean square is a third of what is counted here.  What the matrix cores drop, below
     2^-27 of a running sum, is an eighth of a half step a time.)
     """
